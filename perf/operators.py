@@ -282,10 +282,8 @@ def _decode(c, s, offset, signed):
 def _encode(w, bits, offset, signed):
     """8-bit codes and power-of-two scales of the values `w`; `bits` (16 of them) round each up or down so that its mean stays."""
     q = w.abs().view(-1, BLOCK)
-    e = q.max(1).values.view(torch.int32) >> 23
-    fine = e > 0
-    scale = torch.where(fine, (e << 23).view(torch.float32), 0.0)
-    inv = torch.where(fine, ((254 - e) << 23).view(torch.float32), 0.0)
+    e = (q.max(1).values.view(torch.int32) >> 23).clamp(min=33)      # a scale of 2^-94 at least
+    scale, inv = (e << 23).view(torch.float32), ((254 - e) << 23).view(torch.float32)
     q = (q * inv[:, None]).view(-1)
     least = (1 + 1 / 8) * 2.0 ** ((offset + 1) // 8 - 127)
     bits = bits << 4
