@@ -46,6 +46,40 @@ class Td3Args(C.Structure):
     ]
 
 
+class GatedScanArgs(C.Structure):
+    """struct apx_gated_scan_args (include/apx.h)."""
+    _fields_ = [
+        ("type", C.c_int), ("H", C.c_int), ("T", C.c_int64), ("B", C.c_int64),
+        ("f", c_ptr), ("f_t", C.c_int64), ("f_b", C.c_int64),
+        ("x", c_ptr), ("x_t", C.c_int64), ("x_b", C.c_int64),
+        ("o", c_ptr), ("o_t", C.c_int64), ("o_b", C.c_int64),
+        ("h0", c_ptr), ("reset", c_ptr), ("lens", c_ptr),
+        ("y", c_ptr), ("y_t", C.c_int64), ("y_b", C.c_int64),
+        ("h_last", c_ptr), ("save", c_ptr),
+        ("dy", c_ptr), ("dy_t", C.c_int64), ("dy_b", C.c_int64),
+        ("dh_last", c_ptr),
+        ("df", c_ptr), ("df_t", C.c_int64), ("df_b", C.c_int64),
+        ("dx", c_ptr), ("dx_t", C.c_int64), ("dx_b", C.c_int64),
+        ("do_", c_ptr), ("do_t", C.c_int64), ("do_b", C.c_int64),
+        ("dh0", c_ptr),
+        ("workspace", c_ptr), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class AdamwArgs(C.Structure):
+    """struct apx_adamw_args (include/apx.h)."""
+    _fields_ = [
+        ("n_tensors", C.c_int), ("grad_type", C.c_int), ("state_bits", C.c_int),
+        ("params", c_ptr), ("grads", c_ptr), ("numel", c_ptr), ("weight_decay", c_ptr),
+        ("m", c_ptr), ("v", c_ptr), ("m_scale", c_ptr), ("v_scale", c_ptr),
+        ("t", c_ptr),
+        ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("grad_scale", C.c_double), ("max_norm", C.c_double),
+        ("seed", C.c_uint64),
+        ("workspace", c_ptr), ("workspace_bytes", C.c_size_t),
+        ("norm_out", c_ptr),
+    ]
+
+
 class EnvCfg(C.Structure):
     """struct apx_env_cfg (include/apx.h)."""
     _fields_ = [
@@ -93,6 +127,15 @@ SIGNATURES = {
     "apx_grid_barrier_selftest": (C.c_int, [C.c_int, C.c_int, C.c_int, c_ptr, c_ptr, c_ptr]),
     "apx_clip_adam": (C.c_int, [c_ptr, c_ptr, c_ptr, c_ptr, C.c_int64, C.c_float, C.c_float, C.c_float, C.c_float,
                                 C.c_int, c_ptr, c_ptr]),
+    "apx_gated_scan_save_floats": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int]),
+    "apx_gated_scan_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int]),
+    "apx_gated_scan_forward": (C.c_int, [C.POINTER(GatedScanArgs), c_ptr]),
+    "apx_gated_scan_backward": (C.c_int, [C.POINTER(GatedScanArgs), c_ptr]),
+    "apx_gated_scan_step": (C.c_int, [C.POINTER(GatedScanArgs), c_ptr, c_ptr]),
+    "apx_adamw_state_elements": (C.c_int64, [C.c_int, c_ptr]),
+    "apx_adamw_workspace_bytes": (C.c_size_t, [C.c_int]),
+    "apx_adamw": (C.c_int, [C.POINTER(AdamwArgs), c_ptr]),
+    "apx_adamw_moments": (C.c_int, [c_ptr, c_ptr, c_ptr, c_ptr, C.c_int64, c_ptr, c_ptr, c_ptr]),
     "apx_env_default_cfg": (None, [C.POINTER(EnvCfg)]),
     "apx_env_create": (C.c_int, [C.POINTER(EnvCfg), C.POINTER(c_ptr)]),
     "apx_env_destroy": (C.c_int, [c_ptr]),

@@ -1,0 +1,310 @@
+// One AdamW step over many tensors behind a global-norm clip, moments in 32 or in 8 bits (include/apx.h, apx_adamw).
+//
+//   g = k g;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - step m / (sqrt(v) ibc + eps),  step = lr / (1 - b1^t), ibc = 1 / sqrt(1 - b2^t)
+//
+// Two launches: the first sums the squares of all gradients (one f64 sum per workgroup, its elements in a fixed order) and counts the step, the second adds those sums
+// up again in every workgroup - a few kB out of L2, cheaper than a third launch - and makes the step.  Tensors go into the launches by tables in the kernel arguments
+// (no device copy of pointers that would have to be kept in step with the caller's): up to TABLE tensors a launch.
+// Products and sums of the moments are separate roundings (no fused multiply-add), so that the moments are the same numbers wherever the formula above is evaluated in f32.
+#include "apx_common.h"
+#include <gfx950/half_types.h>
+#include <cmath>
+
+namespace {
+
+using namespace half_types;
+
+constexpr int TABLE = 90;                  // tensors a launch: 40 bytes each, of 4 kB of kernel arguments
+constexpr int BLOCK = 256;                 // elements that share a scale of 8-bit moments, and what a tensor's part of the moments is rounded up to
+constexpr int CHUNK = 2048;                // elements a workgroup takes at a time: 8 blocks
+constexpr int PARTS = 1024;                // partial sums of squares of one launch
+constexpr int GRID = 2048;                 // workgroups of the update at most: 8 for each of 256 CUs
+constexpr unsigned M_OFFSET = 904, V_OFFSET = 776;
+
+struct Table {
+    float* p[TABLE]; const void* g[TABLE]; int64_t n[TABLE];
+    int64_t state[TABLE];                  // where the tensor's moments begin
+    int first[TABLE];                      // its first chunk
+    float wd[TABLE];
+    int tensors, chunks;
+};
+struct Step { float step, ibc; };
+
+// the tensor of a chunk: the last whose first chunk is not beyond it (empty tensors share a first chunk with the next one and are passed over)
+__device__ __forceinline__ int tensor_of(const Table& T, int chunk) {
+    int lo = 0, hi = T.tensors - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (T.first[mid] <= chunk) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+template <int TYPE> __device__ __forceinline__ float grad_at(const void* g, int64_t i) {
+    if constexpr (TYPE == APX_F32) return ((const float*)g)[i];
+    else if constexpr (TYPE == APX_BF16) return widen_bf16(((const uint16_t*)g)[i]);
+    else return widen_f16(((const uint16_t*)g)[i]);
+}
+// sum over the workgroup's 256 threads in a fixed order; every thread gets it
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double part[4];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (part[0] + part[1]) + (part[2] + part[3]);
+    __syncthreads();
+    return v;
+}
+
+__device__ void count_step(int64_t* t, Step* out, double lr, double beta1, double beta2) {
+    const int64_t n = *t + 1;
+    *t = n;
+    out->step = (float)(lr / (1.0 - pow(beta1, (double)n)));
+    out->ibc = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)n)));
+}
+__global__ void adamw_begin_kernel(int64_t* t, Step* out, double lr, double beta1, double beta2) {
+    if (threadIdx.x == 0) count_step(t, out, lr, beta1, beta2);
+}
+template <int TYPE>
+__global__ __launch_bounds__(256) void adamw_norm_kernel(Table T, double* parts, int64_t* t, Step* out, double lr, double beta1, double beta2) {
+    if (t && blockIdx.x == 0 && threadIdx.x == 0) count_step(t, out, lr, beta1, beta2);
+    double sum = 0;
+    for (int chunk = blockIdx.x; chunk < T.chunks; chunk += gridDim.x) {
+        const int k = tensor_of(T, chunk);
+        const int64_t e0 = (int64_t)(chunk - T.first[k]) * CHUNK;
+        const int64_t left = T.n[k] - e0;
+        const int n = left < CHUNK ? (int)left : CHUNK;
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const double g = (double)grad_at<TYPE>(T.g[k], e0 + i);
+            sum += g * g;
+        }
+    }
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) parts[blockIdx.x] = sum;
+}
+
+struct Hyper {
+    float beta1, omb1, beta2, omb2, eps, lr, grad_scale, max_norm;
+    const double* parts; int n_parts;      // 0: no clipping
+    const Step* step; const int64_t* t; uint64_t seed; double* norm_out;
+};
+// what the gradients are multiplied by; false: the norm is not finite
+__device__ __forceinline__ bool clip_factor(const Hyper& P, bool first, float& k) {
+    k = P.grad_scale;
+    if (P.n_parts == 0) return true;
+    double s = 0;
+    for (int i = threadIdx.x; i < P.n_parts; i += 256) s += P.parts[i];
+    const double norm = sqrt(block_sum(s)) * fabs((double)P.grad_scale);
+    if (first && P.norm_out && threadIdx.x == 0) *P.norm_out = norm;
+    const float c = P.max_norm / ((float)norm + 1e-6f);
+    k = (c < 1.f ? c : 1.f) * P.grad_scale;
+    return norm <= 1.7976931348623157e308;
+}
+__device__ __forceinline__ void adam(float g, float& m, float& v, float& p, const Hyper& P, const Step& S, float keep) {
+    m = m * P.beta1 + g * P.omb1;
+    v = v * P.beta2 + (g * g) * P.omb2;
+    // (fast square root and reciprocal, 1 ulp each: 2e-7 of an update, which is itself a small part of p)
+    p = p * keep - S.step * (m * rcp_fast(sqrt_fast(v) * S.ibc + P.eps));
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void adamw32_kernel(Table T, Hyper P, float* __restrict__ M, float* __restrict__ V) {
+    float k;
+    if (!clip_factor(P, blockIdx.x == 0, k)) return;
+    const Step S = *P.step;
+    for (int chunk = blockIdx.x; chunk < T.chunks; chunk += gridDim.x) {
+        const int id = tensor_of(T, chunk);
+        const int64_t e0 = (int64_t)(chunk - T.first[id]) * CHUNK;
+        const int64_t left = T.n[id] - e0;
+        const int n = left < CHUNK ? (int)left : CHUNK;
+        float* p = T.p[id] + e0; float* m = M + T.state[id] + e0; float* v = V + T.state[id] + e0;
+        const float keep = 1.f - P.lr * T.wd[id];
+        for (int i = threadIdx.x; i < n; i += 256) adam(grad_at<TYPE>(T.g[id], e0 + i) * k, m[i], v[i], p[i], P, S, keep);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ 8-bit moments
+__device__ __forceinline__ unsigned mix(unsigned x) {      // 32 bits in which every bit of x has a part (a bijection: xor-shifts and odd factors, taken from the square roots of 2 and 3)
+    x ^= x >> 16; x *= 0x6A09E667u;
+    x ^= x >> 15; x *= 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+__device__ __forceinline__ unsigned step_key(uint64_t seed, int64_t t) {
+    return mix(mix((unsigned)seed) ^ mix((unsigned)(seed >> 32) + 0x3C6EF373u) ^ mix((unsigned)t + 0x54FF53A5u));
+}
+__device__ __forceinline__ unsigned element_noise(unsigned key, int64_t i) { return mix((unsigned)i ^ key ^ ((unsigned)((uint64_t)i >> 32) * 0x3C6EF373u)); }
+
+// s = 2^(the largest's exponent) for a block whose largest |value| has the bits `top`, at least 2^-94 (what the smallest code stands for is a normal number then); NaN for what
+// cannot be held
+__device__ __forceinline__ void block_scale(unsigned top, float& s, float& inv) {
+    unsigned e = top >> 23;
+    e = e < 33u ? 33u : e;
+    s = __uint_as_float(e << 23); inv = __uint_as_float((254u - e) << 23);
+    if (e >= 254) { s = __uint_as_float(0x7fc00000u); inv = 0.f; }
+}
+constexpr float M_LEAST = 1.125f / (1 << 14), V_LEAST = 1.125f / (1 << 30);      // what c = 1 stands for
+__device__ __forceinline__ unsigned encode_m(float m, float inv, unsigned bits16) {
+    const float q = fabsf(m) * inv;      // exact: a power of two
+    const unsigned r = bits16 << 4;
+    unsigned c = ((__float_as_uint(q) + r) >> 20) - M_OFFSET;
+    if (q < M_LEAST) c = (float)r * (M_LEAST / (1 << 20)) < q ? 1u : 0u;
+    return c | (m < 0.f && c ? 128u : 0u);
+}
+__device__ __forceinline__ unsigned encode_v(float v, float inv, unsigned bits16) {
+    const float q = v * inv;
+    unsigned c = ((__float_as_uint(q) + (bits16 << 4)) >> 20) - V_OFFSET;
+    if (q < V_LEAST) c = q > 0.f ? 1u : 0u;
+    return c;
+}
+__device__ __forceinline__ float decode_m(unsigned c, float s) {
+    const float v = ((c & 127u) ? __uint_as_float(((c & 127u) + M_OFFSET) << 20) : 0.f) * s;
+    return (c & 128u) ? -v : v;
+}
+__device__ __forceinline__ float decode_v(unsigned c, float s) { return (c ? __uint_as_float((c + V_OFFSET) << 20) : 0.f) * s; }
+
+// a wave takes a block of 256 elements, a lane 4 of them
+template <int TYPE>
+__global__ __launch_bounds__(256) void adamw8_kernel(Table T, Hyper P, uint8_t* __restrict__ M, uint8_t* __restrict__ V, float* __restrict__ MS, float* __restrict__ VS) {
+    float k;
+    if (!clip_factor(P, blockIdx.x == 0, k)) return;
+    const Step S = *P.step;
+    const unsigned key = step_key(P.seed, *P.t);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int chunk = blockIdx.x; chunk < T.chunks; chunk += gridDim.x) {
+        const int id = tensor_of(T, chunk);
+        const float keep = 1.f - P.lr * T.wd[id];
+        for (int q = wave; q < CHUNK / BLOCK; q += 4) {
+            const int64_t e = (int64_t)(chunk - T.first[id]) * CHUNK + q * BLOCK;
+            if (e >= T.n[id]) break;
+            const int64_t at = T.state[id] + e, blk = at / BLOCK;
+            const float ms = MS[blk], vs = VS[blk];
+            float* p = T.p[id];
+            float m[4], v[4];
+            unsigned mt = 0, vt = 0;
+            for (int i = 0; i < 4; ++i) {
+                const int64_t j = e + lane * 4 + i;
+                m[i] = v[i] = 0.f;
+                if (j < T.n[id]) {
+                    m[i] = decode_m(M[at + lane * 4 + i], ms); v[i] = decode_v(V[at + lane * 4 + i], vs);
+                    adam(grad_at<TYPE>(T.g[id], j) * k, m[i], v[i], p[j], P, S, keep);
+                }
+                const unsigned am = __float_as_uint(m[i]) & 0x7fffffffu, av = __float_as_uint(v[i]) & 0x7fffffffu;      // (as integers: a NaN is larger than all numbers)
+                mt = mt > am ? mt : am; vt = vt > av ? vt : av;
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                const unsigned a = __shfl_xor(mt, o, 64), b = __shfl_xor(vt, o, 64);
+                mt = mt > a ? mt : a; vt = vt > b ? vt : b;
+            }
+            float s, inv, s2, inv2;
+            block_scale(mt, s, inv); block_scale(vt, s2, inv2);
+            for (int i = 0; i < 4; ++i) {
+                const int64_t j = at + lane * 4 + i;
+                const unsigned r = element_noise(key, j);
+                M[j] = (uint8_t)encode_m(m[i], inv, r & 0xffffu);
+                V[j] = (uint8_t)encode_v(v[i], inv2, r >> 16);
+            }
+            if (lane == 0) { MS[blk] = s; VS[blk] = s2; }
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void adamw_moments_kernel(const uint8_t* __restrict__ M, const uint8_t* __restrict__ V, const float* __restrict__ MS, const float* __restrict__ VS,
+                                                            int64_t n, uint16_t* __restrict__ mo, uint16_t* __restrict__ vo) {
+    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        mo[i] = round_bf16(decode_m(M[i], MS[i / BLOCK])); vo[i] = round_bf16(decode_v(V[i], VS[i / BLOCK]));
+    }
+}
+
+struct Workspace { Step* step; double* parts; };
+Workspace workspace_of(void* w) { return {(Step*)w, (double*)((char*)w + 64)}; }
+int launches_of(int n_tensors) { return (n_tensors + TABLE - 1) / TABLE; }
+
+}  // namespace
+
+#define APX_BY_TYPE(type, kernel, grid, block, s, ...)                                                                    \
+    do {                                                                                                                  \
+        if ((type) == APX_F32) hipLaunchKernelGGL(kernel<APX_F32>, dim3(grid), dim3(block), 0, s, __VA_ARGS__);           \
+        else if ((type) == APX_BF16) hipLaunchKernelGGL(kernel<APX_BF16>, dim3(grid), dim3(block), 0, s, __VA_ARGS__);    \
+        else hipLaunchKernelGGL(kernel<APX_F16>, dim3(grid), dim3(block), 0, s, __VA_ARGS__);                             \
+        APX_LAUNCH_CHECK();                                                                                               \
+    } while (0)
+
+extern "C" int64_t apx_adamw_state_elements(int n_tensors, const int64_t* numel) {
+    int64_t n = 0;
+    for (int i = 0; i < n_tensors; ++i) n += numel[i] > 0 ? (numel[i] + BLOCK - 1) / BLOCK * BLOCK : 0;
+    return n;
+}
+extern "C" size_t apx_adamw_workspace_bytes(int n_tensors) { return n_tensors > 0 ? 64 + (size_t)launches_of(n_tensors) * PARTS * sizeof(double) : 0; }
+
+extern "C" int apx_adamw(const apx_adamw_args* a, void* stream) {
+    APX_REQUIRE(a && a->n_tensors >= 0, "args");
+    if (a->n_tensors == 0) return APX_OK;
+    APX_REQUIRE(a->params && a->grads && a->numel && a->t, "null pointer");
+    APX_REQUIRE(a->grad_type == APX_F32 || a->grad_type == APX_BF16 || a->grad_type == APX_F16, "grad_type");
+    APX_REQUIRE(a->state_bits == 32 || a->state_bits == 8, "state_bits");
+    APX_REQUIRE(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1, "beta1, beta2");
+    APX_REQUIRE((float)a->eps >= 1.17549435e-38f && std::isfinite((float)a->eps) && std::isfinite((float)a->lr) && std::isfinite((float)a->grad_scale) && !std::isnan(a->max_norm), "eps, lr, grad_scale, max_norm");
+    int64_t total = 0;
+    for (int i = 0; i < a->n_tensors; ++i) {
+        APX_REQUIRE(a->numel[i] >= 0 && a->numel[i] < ((int64_t)1 << 40), "numel");
+        APX_REQUIRE(a->numel[i] == 0 || (a->params[i] && a->grads[i]), "null tensor");
+        total += a->numel[i];
+    }
+    APX_REQUIRE(total < ((int64_t)1 << 41), "numel in all");
+    APX_REQUIRE(total == 0 || (a->m && a->v && (a->state_bits == 32 || (a->m_scale && a->v_scale))), "moments");
+    APX_REQUIRE(a->workspace && ((uintptr_t)a->workspace & 15) == 0 && a->workspace_bytes >= apx_adamw_workspace_bytes(a->n_tensors), "workspace");
+    const hipStream_t s = (hipStream_t)stream;
+    const Workspace W = workspace_of(a->workspace);
+    const bool clip = a->max_norm > 0;
+    const int n_launches = launches_of(a->n_tensors);
+    auto table = [&](int l, int64_t& state) {
+        Table T;
+        T.tensors = 0; T.chunks = 0;
+        for (int i = l * TABLE; i < a->n_tensors && i < (l + 1) * TABLE; ++i) {
+            const int k = T.tensors++;
+            T.p[k] = a->params[i]; T.g[k] = a->grads[i]; T.n[k] = a->numel[i]; T.state[k] = state; T.first[k] = T.chunks;
+            T.wd[k] = a->weight_decay ? a->weight_decay[i] : 0.f;
+            T.chunks += (int)((a->numel[i] + CHUNK - 1) / CHUNK);
+            state += (a->numel[i] + BLOCK - 1) / BLOCK * BLOCK;
+        }
+        return T;
+    };
+    int n_parts = 0;
+    if (clip) {
+        int64_t state = 0;
+        for (int l = 0; l < n_launches; ++l) {
+            const Table T = table(l, state);
+            const int grid = T.chunks < 1 ? 1 : T.chunks < PARTS ? T.chunks : PARTS;
+            APX_BY_TYPE(a->grad_type, adamw_norm_kernel, grid, 256, s, T, W.parts + n_parts, l == 0 ? a->t : (int64_t*)nullptr, W.step, a->lr, a->beta1, a->beta2);
+            n_parts += grid;
+        }
+    } else {
+        hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(64), 0, s, a->t, W.step, a->lr, a->beta1, a->beta2);
+        APX_LAUNCH_CHECK();
+    }
+    const Hyper P = {(float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps, (float)a->lr, (float)a->grad_scale, (float)a->max_norm,
+                     W.parts, n_parts, W.step, a->t, a->seed, a->norm_out};
+    int64_t state = 0;
+    for (int l = 0; l < n_launches; ++l) {
+        const Table T = table(l, state);
+        if (T.chunks == 0 && l > 0) continue;
+        const int grid = T.chunks < 1 ? 1 : T.chunks < GRID ? T.chunks : GRID;
+        Hyper Q = P;
+        if (l > 0) Q.norm_out = nullptr;
+        if (a->state_bits == 32) APX_BY_TYPE(a->grad_type, adamw32_kernel, grid, 256, s, T, Q, (float*)a->m, (float*)a->v);
+        else APX_BY_TYPE(a->grad_type, adamw8_kernel, grid, 256, s, T, Q, (uint8_t*)a->m, (uint8_t*)a->v, a->m_scale, a->v_scale);
+    }
+    return APX_OK;
+}
+
+extern "C" int apx_adamw_moments(const void* m, const void* v, const float* m_scale, const float* v_scale, int64_t elements, void* m_out, void* v_out, void* stream) {
+    APX_REQUIRE(elements >= 0 && elements % BLOCK == 0, "elements: whole blocks of 256");
+    if (elements == 0) return APX_OK;
+    APX_REQUIRE(m && v && m_scale && v_scale && m_out && v_out, "null pointer");
+    const int64_t want = (elements + 255) / 256;
+    hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)(want < GRID ? want : GRID)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)m, (const uint8_t*)v, m_scale, v_scale,
+                       elements, (uint16_t*)m_out, (uint16_t*)v_out);
+    APX_LAUNCH_CHECK();
+    return APX_OK;
+}

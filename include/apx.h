@@ -123,6 +123,50 @@ int apx_lstm_step(const float* packed, int D, int H, int L, int O, const float* 
 int apx_lstm_backward(const float* params, float* grads, int D, int H, int L, int O, const float* x, int T, int64_t B,
                       const float* save, const float* dy, float* scratch, void* stream);
 
+/* A gated linear recurrence over time-major sequences [T, B, H]: a recurrent core whose gates do not read the state, so that one product over all steps makes them and
+ * the state itself is a scan (beside the LSTM above, whose T steps are a chain of products).  With a = sigmoid(f), n = 1 - a = sigmoid(-f):
+ *   p_t = 0 where reset[t, b] is non-zero, else h_{t-1}            (chosen, not multiplied: whatever the state held does not pass a reset)
+ *   h_t = a_t p_t + n_t x_t          y_t = h_t sigmoid(o_t), or h_t without o
+ * Steps t >= lens[b] (padding behind a trajectory's end) count for nothing: the state stays, y and every gradient there are 0, their inputs may hold anything.
+ * apx_gated_scan_forward:  f, x, o -> y, h_last (the state after the last step; h0 if there is none); save (apx_gated_scan_save_floats floats, or NULL) keeps what the
+ *                          backward pass needs.
+ * apx_gated_scan_backward: the inputs and save of a forward call, dy and dh_last (NULL = 0) -> df, dx, do_ (with o), dh0 (NULL = not wanted).
+ * f, x, o, y, dy, df, dx, do_ hold `type` and lie as strides say, in elements: entry (t, b, j) at t * s_t + b * s_b + j, so f | x | o side by side in the rows of one
+ * product need no copy.  Inputs may overlap or repeat (stride 0); outputs must not overlap each other or an input, nor themselves.  h0, h_last, save, dh_last, dh0: f32,
+ * dense [B, H].  reset: u8, dense [T, B].  lens: i32 [B], below 0 taken as 0 and above T as T.  States, gates and sums are f32 whatever the type; each output is rounded once.
+ * workspace: apx_gated_scan_workspace_bytes bytes (0 for most shapes: then it may be NULL), 16-byte aligned, not shared by calls that may run at the same time.
+ * Results do not depend on anything but the inputs and shapes (no atomics).  T = 0, B = 0 and H = 0 are allowed. all pointers [dev] */
+#define APX_F32 0
+#define APX_BF16 1
+#define APX_F16 2
+typedef struct apx_gated_scan_args {
+    int type, H;
+    int64_t T, B;
+    const void* f; int64_t f_t, f_b;
+    const void* x; int64_t x_t, x_b;
+    const void* o; int64_t o_t, o_b;               /* NULL: no output gate */
+    const float* h0;                               /* NULL: zero start */
+    const uint8_t* reset;                          /* NULL: none */
+    const int32_t* lens;                           /* NULL: every step counts */
+    void* y; int64_t y_t, y_b;                     /* forward */
+    float* h_last;
+    float* save;
+    const void* dy; int64_t dy_t, dy_b;            /* backward */
+    const float* dh_last;
+    void* df; int64_t df_t, df_b;
+    void* dx; int64_t dx_t, dx_b;
+    void* do_; int64_t do_t, do_b;
+    float* dh0;
+    void* workspace; size_t workspace_bytes;
+} apx_gated_scan_args;
+size_t apx_gated_scan_save_floats(int64_t T, int64_t B, int H);
+size_t apx_gated_scan_workspace_bytes(int64_t T, int64_t B, int H);
+int apx_gated_scan_forward(const apx_gated_scan_args* args, void* stream);
+int apx_gated_scan_backward(const apx_gated_scan_args* args, void* stream);
+/* One step of the same recurrence, for the rollout: h [B, H] f32 (dense) is updated in place, y [B, H] = the step's output; rows of f, x, o, y lie f_b, x_b, o_b, y_b
+ * elements apart; rows whose reset byte ([B]) is non-zero start from a zero state.  T, lens, save and the backward fields are not read. */
+int apx_gated_scan_step(const apx_gated_scan_args* args, float* h, void* stream);
+
 /* The padded minibatch of the recurrent update (rl/algos/ppo.py:411-430: pad_sequence over the sampled trajectories, zero rows behind a trajectory's end) gathered out of
  * the rollout grid in one launch.  Which grid row column b holds at step t: either idx [T, B] int64 (flat grid row, -1 = padded), or - idx NULL - the trajectory list
  * traj [n_traj, 3] int64 = (grid column n, t0, t1) with sel [B] int64 (NULL: 0..B-1) naming column b's trajectory and N = the grid's column count: step t of the
@@ -220,6 +264,43 @@ int apx_grid_barrier_selftest(int workgroups, int phases, int n_words, unsigned*
  * on an (all-reduced) gradient; scale multiplies the gradient first (1/world_size for an averaged sum). */
 int apx_clip_adam(float* param, float* m, float* v, float* grad, int64_t n, float grad_scale, float grad_clip,
                   float lr, float adam_eps, int adam_t, double* sumsq_scratch, void* stream);
+
+/* One AdamW step (decoupled weight decay) over any number of tensors, behind a global-norm clip over all of them: apx_clip_adam serves one flat block per call, this the
+ * tensors of a network where they lie, each with its own weight decay, moments in 32 or in 8 bits.
+ *   N = |grad_scale| sqrt(sum of g^2 over all tensors)          k = grad_scale min(1, max_norm / (N + 1e-6))      (torch.nn.utils.clip_grad_norm_)
+ *   g = k g      m = beta1 m + (1 - beta1) g      v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * max_norm <= 0: no clipping (k = grad_scale, N is not formed, norm_out is not written).  With clipping a step whose N is infinite or NaN changes neither parameters nor
+ * moments (t still counts it); norm_out shows it.
+ * 0 <= beta < 1, eps > 0 (a normal f32: the update of a moment that is still 0 is 0, not 0 / 0).
+ * params / grads / numel / weight_decay: [host] arrays of n_tensors entries (weight_decay NULL: 0); the tensors dense, parameters f32, gradients grad_type.  Tensors must not
+ * overlap.  Empty tensors are allowed.
+ * Moments: one flat block each for m and v, in the tensors' order, every tensor's part starting at a multiple of 256 elements (apx_adamw_state_elements in all); zero before
+ * the first step.  state_bits 32: f32.  state_bits 8: one u8 code per element and one f32 scale per 256 elements of a tensor (m_scale, v_scale), a power of two s >= 2^-94 with
+ * max|.| in [s, 2 s), or below s = 2^-94.  An m code is a sign bit above a 7-bit c, a v code an 8-bit c; c stands for 0 if c = 0, else for s times the f32 number with the bits (c + 904) << 20 (m)
+ * or (c + 776) << 20 (v): 1/8 of its power of two apart, down to 2^-14 s (m) and 2^-30 s (v).  Values are rounded up or down by 16 pseudo-random bits of (seed, t, element)
+ * with the probability that keeps their mean (rounded to nearest, a v that moves by 1 - beta2 of itself a step would never leave its code); a v > 0 below the range takes the
+ * smallest code, not 0.  A block that holds an infinity, a NaN or a value of 2^127 and more reads back as NaN.  The update itself uses the moments before this rounding.
+ * t: i64 [dev], the steps taken so far, counted up here (so that a captured step counts when it is replayed).
+ * workspace: apx_adamw_workspace_bytes bytes, 16-byte aligned.  params / grads / m / v may have any alignment their type allows.  Sums run in a fixed order (no atomics).
+ * apx_adamw_moments: 8-bit moments as the values they stand for, in bf16 (which holds them exactly). */
+typedef struct apx_adamw_args {
+    int n_tensors, grad_type, state_bits;
+    float* const* params;
+    const void* const* grads;
+    const int64_t* numel;
+    const float* weight_decay;
+    void* m; void* v; float* m_scale; float* v_scale;
+    int64_t* t;
+    double lr, beta1, beta2, eps, grad_scale, max_norm;
+    uint64_t seed;
+    void* workspace; size_t workspace_bytes;
+    double* norm_out;                              /* f64 [dev] or NULL */
+} apx_adamw_args;
+int64_t apx_adamw_state_elements(int n_tensors, const int64_t* numel);
+size_t apx_adamw_workspace_bytes(int n_tensors);
+int apx_adamw(const apx_adamw_args* args, void* stream);
+int apx_adamw_moments(const void* m, const void* v, const float* m_scale, const float* v_scale, int64_t elements, void* m_out, void* v_out, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------
  * Environment half: batched Cassie-v0.  Replaces the per-env FFI of cassie/cassiemujoco/cassiemujoco.py:33-336

@@ -1,0 +1,210 @@
+"""Bodies of the sequence operators' tests: tests/test_gpu_sequence.py runs them on the GPU, tests/test_kernel_emulation_sequence.py on the kernels' sources compiled for the host.
+The oracle is oracle/sequence.py in 64 bits.
+
+Tolerances (u = 2^-24, half a step of f32 relative to the value; fast exponential and reciprocal: 2u each):
+ * a gate's smaller half lo = e / (1 + e), e = 2^(-|f| log2 e): the argument's rounding moves e by |f| u, the exponential by 2u, the sum by u, the reciprocal by 2u, the product by u
+   -> delta = (|f| + 6) u relative; the larger half is 1 - lo, u more.
+ * h_t = a h + n x: the gates' error counts n delta (|h| + |x|) a step, sum and fma 2u |h| a step, and each fades with the memory: sum_k a^k n <= 1, sum_k a^k <= L =
+   min(T, 1 / min n).  With M = max(|x|, |h0|): |error of h| <= M (2 delta + 4 u L).  Steps may be joined in chunks: the product of a chunk's a carries (chunk) u more, counted the
+   same way: twice the bound.
+ * g_t = d_t + a g: the same with G = max |g|: |error of g| <= 2 G (2 delta + 4 u L).
+ * outputs: dx = n g, df = g (p - x) a n, do = d h s r with |a n|, |s r| <= 1/4, |p - x| <= 2 M; y = h s.  8 more roundings of u.  And half a step of the output's own type."""
+import numpy as np
+import torch
+
+from oracle import sequence as Q
+
+U = 2.0 ** -24
+NP = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def half_step(t):
+    return torch.finfo(NP[t]).eps / 2
+
+
+def smallest(t):
+    return 2.0 ** -25 if t == "f16" else 2.0 ** -134 if t == "bf16" else 0.0      # half a step of the numbers below the smallest normal one
+
+
+def make(T, B, H, t, gate, reset, lens, carry, dev, seed, lean=1.0, layout="rows"):
+    """inputs on the device, rounded to their type, and the same values in 64 bits"""
+    r = np.random.RandomState(seed)
+    k = 3 if gate else 2
+    proj = r.randn(T, B, k * H) * 1.5
+    proj[..., :H] = np.clip(proj[..., :H] + lean, -6, 6)
+    proj = torch.tensor(proj, dtype=torch.float32).to(NP[t]).to(dev)
+    parts = [proj[..., i * H:(i + 1) * H] for i in range(k)]
+    if layout == "dense":
+        parts = [p.contiguous() for p in parts]
+    elif layout == "batch first":
+        parts = [p.permute(1, 0, 2).contiguous().permute(1, 0, 2) for p in parts]
+    elif layout == "shifted":      # rows that begin off every wide load's alignment
+        parts = [torch.cat([p.new_zeros(T, B, 1), p], 2)[..., 1:] for p in parts]
+    d = dict(f=parts[0], x=parts[1], o=parts[2] if gate else None,
+             h0=torch.tensor(r.randn(B, H), dtype=torch.float32, device=dev) if carry else None,
+             reset=torch.tensor((r.rand(T, B) < 0.15).astype(np.uint8), device=dev) if reset else None,
+             lens=torch.tensor(r.randint(0, T + 1, B).astype(np.int32), device=dev) if lens else None)
+    dy = torch.tensor(r.randn(T, B, H), dtype=torch.float32).to(NP[t]).to(dev)
+    dh = torch.tensor(r.randn(B, H), dtype=torch.float32, device=dev) if carry else None
+    return d, dy, dh
+
+
+def f64(t):
+    return None if t is None else t.detach().cpu().double().numpy() if t.is_floating_point() else t.detach().cpu().numpy()
+
+
+def wide(d):
+    return {k: f64(v) for k, v in d.items()}
+
+
+def bounds(d, G=0.0, D=0.0):
+    """(error of h, error of g, delta, M) of the derivation above; only what counts enters: padding may hold anything"""
+    w = wide(d)
+    T = w["f"].shape[0]
+    live = np.ones(w["f"].shape[:2], bool) if w["lens"] is None else np.arange(T)[:, None] < w["lens"][None]
+    f, x = w["f"][live], w["x"][live]
+    if f.size == 0:
+        return U, U, U, float(np.abs(w["h0"]).max()) if w["h0"] is not None and w["h0"].size else 0.0
+    fin = np.abs(f[np.isfinite(f)])
+    top = float(fin.max()) if fin.size else 0.0
+    delta = (min(top, 100.0) + 6) * U
+    L = min(T, 1 / max(float(Q.sigmoid(-f).min()), 1e-30))
+    M = max(float(np.abs(x).max()), float(np.abs(w["h0"]).max()) if w["h0"] is not None else 0.0)
+    return 2 * M * (2 * delta + 4 * U * L), 2 * G * (2 * delta + 4 * U * L), delta, M
+
+
+def close(name, got, ref, tol, t):
+    got = f64(got)
+    assert np.isfinite(got).all(), (name, "not finite")
+    err = np.abs(got - ref) - half_step(t) * np.abs(ref) * (1 + 1e-3) - smallest(t)
+    assert got.shape == ref.shape and (got.size == 0 or err.max() <= tol), (name, float(err.max()), tol)
+
+
+def check_scan(dev, T, B, H, t="f32", gate=False, reset=False, lens=False, carry=False, seed=0, lean=1.0, layout="rows", poison=False):
+    from apex_amd import engine
+    d, dy, dh = make(T, B, H, t, gate, reset, lens, carry, dev, seed, lean, layout)
+    if poison:      # what must not count holds NaN and infinities: padding behind the ends, states in front of a reset
+        assert lens and reset and carry
+        n = d["lens"].cpu().numpy()
+        for b in range(B):
+            for k in ("f", "x", "o"):
+                if d[k] is not None:
+                    d[k][n[b]:, b] = [float("nan"), float("inf"), -float("inf"), torch.finfo(NP[t]).min][b % 4]
+            dy[n[b]:, b] = float("nan")
+            if n[b] > 0:
+                d["reset"][0, b] = 1
+                d["h0"][b] = float("nan") if b % 2 else float("inf")
+    w = wide(d)
+    keep_inputs = {k: v.clone() for k, v in d.items() if v is not None}
+    y, hs, _, h = Q.gated_scan(**w)
+    df, dx, do, dh0, G = Q.gated_scan_grad(dy=f64(dy), dh_last=f64(dh), **w)
+    if poison:
+        rows = n > 0
+        d2 = dict(d, h0=torch.where(torch.tensor(rows, device=dev)[:, None], torch.zeros_like(d["h0"]), d["h0"]))
+        eh, eg, delta, M = bounds(d2, G)
+    else:
+        eh, eg, delta, M = bounds(d, G)
+    gy, gh, save = engine.gated_scan(**d, keep=True)
+    y2, h2 = engine.gated_scan(**d)
+    assert torch.equal(gy, y2) and torch.equal(gh, h2), "keep=True changes the outputs"
+    close("y", gy, y, eh + 3 * U * M, t)
+    close("h_last", gh, h, eh, "f32")
+    out = engine.gated_scan_backward(d["f"], d["x"], dy, save, o=d["o"], h0=d["h0"], reset=d["reset"], lens=d["lens"], dh_last=dh)
+    D = float(np.abs(f64(dy)[np.isfinite(f64(dy))]).max()) if dy.numel() else 0.0
+    close("df", out[0], df, 0.25 * (2 * M * eg + G * 2 * eh) + 0.5 * M * G * (2 * delta + 8 * U), t)
+    close("dx", out[1], dx, eg + G * (delta + 8 * U), t)
+    if gate:
+        close("do", out[2], do, 0.25 * D * eh + 0.25 * D * M * (2 * delta + 8 * U), t)
+    else:
+        assert out[2] is None
+    if carry:
+        fin = np.isfinite(dh0)
+        assert fin.all()
+        close("dh0", out[3], dh0, eg + 4 * U * max(G, 1.0), "f32")
+    else:
+        assert out[3] is None
+    for k, v in keep_inputs.items():
+        assert torch.equal(torch.nan_to_num(v.float()), torch.nan_to_num(d[k].float())), "input %s was written" % k
+    return gy, gh, out
+
+
+def check_step(dev, B, H, t="f32", gate=False, reset=False, seed=0, layout="rows", steps=3):
+    """steps of gated_scan_step against one gated_scan over the same inputs in 64 bits"""
+    from apex_amd import engine
+    d, _, _ = make(steps, B, H, t, gate, reset, False, True, dev, seed, 1.0, layout)
+    y, hs, _, _ = Q.gated_scan(**wide(d))
+    eh, _, _, M = bounds(d)
+    h = d["h0"].clone()
+    for k in range(steps):
+        got = engine.gated_scan_step(d["f"][k], d["x"][k], h, o=None if d["o"] is None else d["o"][k], reset=None if d["reset"] is None else d["reset"][k])
+        close("y", got, y[k], eh + 3 * U * M, t)
+        close("h", h, hs[k], eh, "f32")
+
+
+# ------------------------------------------------------------------------------------------------ AdamW
+def check_adamw(dev, shapes, bits=32, grad="f32", clip=None, steps=3, seed=0, wd=0.01, scale=1.0, flat=False, sizes=1.0):
+    """steps of AdamW against the 64-bit oracle: 32-bit moments and the parameters to a few roundings, 8-bit moments code by code.
+    Moments: g k (k: 4u), one product each and one sum -> (6 + 3 a step) u relative to the largest summand.  Parameters a step: 3u |p| for decay and difference, and of the
+    update |step m / den| (m: (6 + 3 steps) u, square root of v, products, reciprocal: 12 u): (20 + 6 steps) u lr U with U the update's size, at most |m_hat| / eps."""
+    from apex_amd import engine
+    r = np.random.RandomState(seed)
+    hyper = dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-5)
+    ns = [int(np.prod(s)) for s in shapes]
+    if flat:
+        block = torch.tensor(r.randn(sum(ns)) * 0.1, dtype=torch.float32).to(dev)
+        ps, at = [], 0
+        for s, n in zip(shapes, ns):
+            ps.append(block[at:at + n].view(*s)); at += n
+    else:
+        ps = [torch.tensor(r.randn(*s) * 0.1, dtype=torch.float32).to(dev) for s in shapes]
+    decay = [wd if k % 2 == 0 else 0.0 for k in range(len(shapes))]
+    opt = engine.AdamW(ps, weight_decay=decay, max_norm=clip, state_bits=bits, seed=seed + (5 << 32), **hyper)
+    where, total = Q.layout(ns)
+    assert opt.elements == total
+    P = [f64(p).reshape(-1) for p in ps]
+    M, V = np.zeros(total), np.zeros(total)
+    M32, V32 = np.zeros(total, np.float32), np.zeros(total, np.float32)
+    spread = 0.0
+    for t in range(1, steps + 1):
+        g = [torch.tensor(r.randn(*s) * sizes * 10.0 ** (-(i % 4)) * (r.rand(*s) > 0.05), dtype=torch.float32).to(NP[grad]).to(dev) for i, s in enumerate(shapes)]
+        opt.step(g, grad_scale=scale)
+        g64 = [f64(x).reshape(-1) for x in g]
+        norm, k = Q.clip_factor(g64, scale, clip)
+        if clip:
+            assert abs(float(opt.norm) - norm) <= 1e-12 * norm
+        k32 = np.float32(scale) if not clip else np.float32(min(np.float32(1), np.float32(clip) / (np.float32(norm) + np.float32(1e-6)))) * np.float32(scale)
+        full = np.zeros(total, np.float32)
+        for i, n in enumerate(ns):
+            full[where[i]:where[i] + n] = g64[i].astype(np.float32)
+        if bits == 8:      # the moments before their rounding, from the codes that were there
+            M, V = M32.astype(np.float64), V32.astype(np.float64)
+        M32n, V32n = Q.moments_f32(full, M32, V32, hyper["betas"][0], hyper["betas"][1], k32)
+        for i, n in enumerate(ns):
+            s = slice(where[i], where[i] + n)
+            p, M[s], V[s] = Q.adamw(P[i], g64[i], M[s], V[s], t, hyper["lr"], *hyper["betas"], hyper["eps"], decay[i], k)
+            upd = np.abs(p - P[i]).max() if n else 0.0
+            spread += 3 * U * (np.abs(P[i]).max() if n else 0.0) + (20 + 6 * t) * U * upd
+            P[i] = p
+            got = f64(ps[i]).reshape(-1)
+            assert n == 0 or np.abs(got - p).max() <= spread, ("p", i, t, np.abs(got - p).max(), spread)
+        if bits == 32:
+            M32, V32 = M32n, V32n
+            assert np.array_equal(opt.m.cpu().numpy(), M32) and np.array_equal(opt.v.cpu().numpy(), V32), "moments differ from separate f32 roundings"
+            assert np.abs(M32 - M).max() <= (6 + 3 * t) * U * np.abs(M).max() and np.abs(V32 - V).max() <= (12 + 3 * t) * U * np.abs(V).max()
+        else:
+            rnd = Q.noise(seed + (5 << 32), t, np.arange(total))
+            mc, ms = Q.encode(M32n, rnd & np.uint64(0xffff), Q.M_OFFSET, True)
+            vc, vs = Q.encode(V32n, rnd >> np.uint64(16), Q.V_OFFSET, False)
+            assert np.array_equal(opt.m_scale.cpu().numpy(), ms) and np.array_equal(opt.v_scale.cpu().numpy(), vs)
+            assert np.array_equal(opt.m.cpu().numpy(), mc) and np.array_equal(opt.v.cpu().numpy(), vc)
+            M32, V32 = Q.decode(mc, ms, Q.M_OFFSET, True).astype(np.float32), Q.decode(vc, vs, Q.V_OFFSET, False).astype(np.float32)
+            # at most one step of the code (an eighth of the value's power of two) from the moment, below the range at most its smallest number
+            sm, sv = np.repeat(ms, Q.BLOCK), np.repeat(vs, Q.BLOCK)
+            assert (np.abs(M32 - M32n) <= np.maximum(np.abs(M32n) / 8, sm * 2.0 ** -13)).all() and (np.abs(V32 - V32n) <= np.maximum(V32n / 8, sv * 2.0 ** -29)).all()
+            assert ((V32n > 0) == (V32 > 0)).all()
+            got = opt.moments()
+            assert np.array_equal(f64(got[0]), M32.astype(np.float64)) and np.array_equal(f64(got[1]), V32.astype(np.float64))
+        assert int(opt.t) == t
+    for v, p in zip(opt.views(opt.moments()[0]), ps):
+        assert v.shape == p.shape
+    return opt, ps

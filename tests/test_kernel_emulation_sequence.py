@@ -1,0 +1,186 @@
+"""CPU: the sequence operators' kernel SOURCES (apex_amd/csrc/gated_scan.hip, adamw.hip) compiled for the host under tools/hipemu, through the host code of apex_amd/engine.py and the
+bodies of the GPU tests (tests/sequence_bodies.py), and the refusals of both layers (which end before anything is launched)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from tests import sequence_bodies as S
+from tests.test_kernel_emulation_learner import dev  # noqa: F401  (the fixture that puts the emulated library in place)
+
+SCANS = [
+    dict(T=1, B=1, H=1), dict(T=1, B=3, H=5, gate=True, reset=True, lens=True, carry=True), dict(T=7, B=2, H=3, carry=True), dict(T=16, B=1, H=64, gate=True),
+    dict(T=17, B=3, H=21, reset=True, carry=True), dict(T=33, B=2, H=40, t="bf16", gate=True, lens=True, carry=True), dict(T=50, B=3, H=17, t="f16", reset=True, lens=True, carry=True),
+    dict(T=40, B=5, H=13, gate=True, reset=True, lens=True, carry=True, poison=True), dict(T=300, B=1, H=8, reset=True, carry=True, lean=4.0), dict(T=130, B=1, H=65, t="bf16", gate=True),
+    dict(T=70, B=2, H=16, gate=True, lens=True, layout="batch first"), dict(T=20, B=2, H=12, gate=True, carry=True, layout="shifted"), dict(T=21, B=2, H=12, t="bf16", layout="dense"),
+]
+
+
+@pytest.mark.parametrize("case", SCANS, ids=lambda c: "-".join("%s%s" % kv for kv in c.items()))
+def test_emulated_scan(dev, case):  # noqa: F811
+    S.check_scan(dev, **case)
+
+
+def test_emulated_scan_of_nothing(dev):  # noqa: F811
+    from apex_amd import engine
+    h0 = torch.randn(3, 4)
+    y, h, save = engine.gated_scan(torch.zeros(0, 3, 4), torch.zeros(0, 3, 4), h0=h0, keep=True)
+    assert y.shape == (0, 3, 4) and torch.equal(h, h0) and save.numel() == 0
+    dh = torch.randn(3, 4)
+    df, dx, do, dh0 = engine.gated_scan_backward(torch.zeros(0, 3, 4), torch.zeros(0, 3, 4), torch.zeros(0, 3, 4), save, h0=h0, dh_last=dh)
+    assert df.shape == (0, 3, 4) and torch.equal(dh0, dh)
+    for shape in ((5, 0, 4), (5, 3, 0)):
+        y, h = engine.gated_scan(torch.zeros(*shape), torch.zeros(*shape))
+        assert y.shape == shape and h.shape == shape[1:]
+    f = torch.randn(6, 2, 4)
+    y, h = engine.gated_scan(f, f, h0=h0[:2].contiguous(), lens=torch.tensor([0, -5], dtype=torch.int32))
+    assert torch.equal(h, h0[:2]) and not y.any()
+    a, b = engine.gated_scan(f, f), engine.gated_scan(f, f, lens=torch.tensor([6, 2 ** 31 - 1], dtype=torch.int32))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("case", [dict(B=1, H=1), dict(B=5, H=13, gate=True, reset=True), dict(B=3, H=64, t="bf16", gate=True), dict(B=4, H=8, t="f16", reset=True),
+                                  dict(B=3, H=12, gate=True, layout="shifted")], ids=str)
+def test_emulated_step(dev, case):  # noqa: F811
+    S.check_step(dev, **case)
+
+
+ADAMW = [
+    dict(shapes=[(1,)], clip=0.05), dict(shapes=[(5, 7), (3,), (257,), (16, 16)], clip=0.05, flat=True), dict(shapes=[(300,), (0,), (1,)], grad="bf16"),
+    dict(shapes=[(1,)], bits=8), dict(shapes=[(5, 7), (3,), (257,), (16, 16)], bits=8, clip=0.05, flat=True, scale=0.5), dict(shapes=[(2100,), (0,), (1,)], bits=8, grad="f16", clip=10.0),
+    dict(shapes=[(256, 4), (64,)], bits=8, sizes=1e-18), dict(shapes=[(300,)], bits=8, sizes=1e-36),
+    dict(shapes=[(k % 5 + 1,) for k in range(200)], bits=8, clip=0.01, steps=2), dict(shapes=[(k % 5 + 1,) for k in range(91)], clip=0.01, steps=2),
+]
+
+
+@pytest.mark.parametrize("case", ADAMW, ids=lambda c: "%d-%s" % (len(c["shapes"]), c.get("bits", 32)))
+def test_emulated_adamw(dev, case):  # noqa: F811
+    S.check_adamw(dev, **case)
+
+
+def test_emulated_adamw_special_blocks(dev):  # noqa: F811
+    """A norm that is not finite changes nothing but the count; without clipping an infinity or a NaN stays in its block; a block of zeros stays zero."""
+    from apex_amd import engine
+    p = [torch.ones(300), torch.ones(5)]
+    o = engine.AdamW(p, max_norm=1.0, state_bits=8)
+    o.step([torch.full((300,), float("inf")), torch.ones(5)])
+    assert torch.equal(p[0], torch.ones(300)) and torch.equal(p[1], torch.ones(5)) and not o.m.any() and not o.v.any() and int(o.t) == 1 and float(o.norm) == float("inf")
+    o = engine.AdamW(p, state_bits=8)
+    g = torch.zeros(300); g[3] = float("nan")
+    o.step([g, torch.zeros(5)])
+    m, v = o.moments()
+    assert torch.isnan(m[:256]).all() and not m[256:].any() and not v[256:].any() and torch.isnan(p[0][3]) and torch.isfinite(p[0][4:]).all() and torch.equal(p[1], torch.ones(5))
+
+
+def test_emulated_adamw_rounding_keeps_the_mean(dev):  # noqa: F811
+    """4096 elements that all hold the same moments: m = 0.1 g, v = 0.001 g^2 in the first step, rounded up or down to neighbours an eighth of a power of two apart.  The mean of n
+    independent roundings is off by at most (step / 2) / sqrt(n) in the standard deviation: five of them here."""
+    from apex_amd import engine
+    n = 4096
+    for g in (0.3, 1.234, 0.0777):
+        o = engine.AdamW([torch.zeros(n)], state_bits=8, seed=11)
+        o.step([torch.full((n,), g)])
+        m, v = o.moments()
+        for got, want in ((m.double(), 0.1 * g), (v.double(), 0.001 * g * g)):
+            step = 2.0 ** np.floor(np.log2(want)) / 8
+            assert abs(float(got.mean()) - want) < 5 * step / 2 / np.sqrt(n)
+            assert len(torch.unique(got)) <= 2
+
+
+# ------------------------------------------------------------------------------------------------ refusals (no device needed: they come before any launch)
+def test_refusals_of_the_wrappers(dev):  # noqa: F811
+    from apex_amd import engine
+    f, x = torch.zeros(4, 2, 3), torch.zeros(4, 2, 3)
+    bad = [
+        lambda: engine.gated_scan(f[0], x[0]), lambda: engine.gated_scan(f.double(), x.double()), lambda: engine.gated_scan(f, x[:3]), lambda: engine.gated_scan(f, x.bfloat16()),
+        lambda: engine.gated_scan(f, x, o=x[..., :2]), lambda: engine.gated_scan(f, x, h0=torch.zeros(2, 4)), lambda: engine.gated_scan(f, x, h0=torch.zeros(2, 3).bfloat16()),
+        lambda: engine.gated_scan(f, x, reset=torch.zeros(4, 2)), lambda: engine.gated_scan(f, x, reset=torch.zeros(2, 4, dtype=torch.uint8)),
+        lambda: engine.gated_scan(f, x, lens=torch.zeros(2, dtype=torch.int64)), lambda: engine.gated_scan(f, x, lens=torch.zeros(3, dtype=torch.int32)),
+        lambda: engine.gated_scan(f, x, out=x), lambda: engine.gated_scan(f, x, out=torch.zeros(4, 2, 3, dtype=torch.float16)), lambda: engine.gated_scan(f, x, out=torch.zeros(1, 1, 3).expand(4, 2, 3)),
+        lambda: engine.gated_scan(f, x, out=torch.zeros(4, 2, 6)[..., ::2]),
+        lambda: engine.gated_scan_step(f, x, torch.zeros(2, 3)), lambda: engine.gated_scan_step(f[0], x[0], torch.zeros(2, 3).bfloat16()), lambda: engine.gated_scan_step(f[0], x[0], torch.zeros(3, 2).t()),
+        lambda: engine.gated_scan_step(f[0], x[0], torch.zeros(2, 3), reset=torch.zeros(3, dtype=torch.uint8)),
+    ]
+    _, _, save = engine.gated_scan(f, x, keep=True)
+    bad += [lambda: engine.gated_scan_backward(f, x, x[:3], save), lambda: engine.gated_scan_backward(f, x, x, save[:-1]), lambda: engine.gated_scan_backward(f, x, x, save.double()),
+            lambda: engine.gated_scan_backward(f, x, x, save, out=(torch.zeros(4, 2, 3),)), lambda: engine.gated_scan_backward(f, x, x, save, dh_last=torch.zeros(3, 2))]
+    t = torch.zeros(4, 2, 3)
+    bad += [lambda: engine.gated_scan_backward(f, x, x, save, out=(t, t)), lambda: engine.gated_scan_backward(f, x, torch.ones(4, 2, 3), save, out=(t, f))]
+    p = [torch.zeros(3), torch.zeros(4)]
+    bad += [lambda: engine.AdamW([]), lambda: engine.AdamW([torch.zeros(3).double()]), lambda: engine.AdamW([torch.zeros(3, 4).t()]), lambda: engine.AdamW(p, state_bits=16),
+            lambda: engine.AdamW(p, weight_decay=[0.1])]
+    o = engine.AdamW(p)
+    bad += [lambda: o.step([torch.zeros(3)]), lambda: o.step([torch.zeros(3), torch.zeros(5)]), lambda: o.step([torch.zeros(3), torch.zeros(4).bfloat16()]),
+            lambda: o.step([torch.zeros(3).double(), torch.zeros(4).double()]), lambda: o.step([torch.zeros(6)[::2], torch.zeros(4)]),
+            lambda: engine.AdamW(p, eps=0.0).step([torch.zeros(3), torch.zeros(4)]), lambda: engine.AdamW(p, betas=(1.0, 0.9)).step([torch.zeros(3), torch.zeros(4)]),
+            lambda: engine.AdamW(p, lr=float("nan")).step([torch.zeros(3), torch.zeros(4)])]
+    for i, call in enumerate(bad):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()
+            pytest.fail("call %d was taken" % i)
+    assert not p[0].any() and int(o.t) == 0
+
+
+def test_refusals_of_the_c_entry_points():
+    """apx_* of the product library itself: every refusal returns APX_E_ARG with a message and launches nothing (there is no device here)."""
+    from apex_amd import _lib
+    lib = _lib.load()
+    one = 16      # a pointer that is never followed: each call below is refused before
+
+    def scan(fn, **change):
+        a = _lib.GatedScanArgs(type=0, H=4, T=3, B=2, f=one, f_t=8, f_b=4, x=2 * one, x_t=8, x_b=4, y=3 * one, y_t=8, y_b=4, h_last=4 * one, dy=5 * one, dy_t=8, dy_b=4, df=6 * one, df_t=8, df_b=4,
+                               dx=7 * one, dx_t=8, dx_b=4, save=8 * one)
+        for k, v in change.items():
+            setattr(a, k, v)
+        return fn(C.byref(a), None)
+    F, Bk = lib.apx_gated_scan_forward, lib.apx_gated_scan_backward
+    calls = [scan(F, type=3), scan(F, type=-1), scan(F, T=-1), scan(F, B=-1), scan(F, H=-1), scan(F, f=None), scan(F, x=None), scan(F, y=None), scan(F, h_last=None),
+             scan(F, f_t=-8), scan(F, y_b=3), scan(F, y_t=7), scan(F, y_t=0), scan(F, y=one), scan(F, h0=4 * one), scan(F, o=9 * one, o_t=-1), scan(F, T=1 << 58), scan(F, B=1 << 35),
+             scan(F, f_t=1 << 60), scan(Bk, save=None), scan(Bk, dy=None), scan(Bk, df=7 * one), scan(Bk, df=one), scan(Bk, o=9 * one, o_t=8, o_b=4), scan(Bk, dx_b=0),
+             scan(Bk, dh0=11 * one, dh_last=11 * one)]
+    s = _lib.GatedScanArgs(type=0, H=4, B=2, f=one, f_b=4, x=2 * one, x_b=4, y=3 * one, y_b=4)
+    calls.append(lib.apx_gated_scan_step(C.byref(s), None, None))
+    s.y_b = 2
+    calls.append(lib.apx_gated_scan_step(C.byref(s), 4 * one, None))
+    calls += [lib.apx_gated_scan_step(None, 4 * one, None), F(None, None), Bk(None, None), lib.apx_adamw(None, None)]
+
+    def adam(**change):
+        ptr, num, wd = (C.c_void_p * 1)(one), (C.c_int64 * 1)(5), None
+        a = _lib.AdamwArgs(n_tensors=1, grad_type=0, state_bits=32, params=C.addressof(ptr), grads=C.addressof(ptr), numel=C.addressof(num), m=2 * one, v=3 * one, t=4 * one, lr=1e-3, beta1=0.9,
+                           beta2=0.999, eps=1e-8, grad_scale=1.0, max_norm=0.0, workspace=5 * one, workspace_bytes=1 << 20)
+        if "num" in change:
+            num[0] = change.pop("num")
+        if "null" in change:
+            ptr[0] = change.pop("null")
+        for k, v in change.items():
+            setattr(a, k, v)
+        return lib.apx_adamw(C.byref(a), None)
+    nan, inf = float("nan"), float("inf")
+    calls += [adam(n_tensors=-1), adam(params=None), adam(grads=None), adam(numel=None), adam(t=None), adam(grad_type=3), adam(state_bits=4), adam(beta1=1.0), adam(beta2=-0.1), adam(beta1=nan),
+              adam(eps=0.0), adam(eps=-1.0), adam(eps=1e-46), adam(eps=nan), adam(lr=inf), adam(lr=1e39), adam(grad_scale=nan), adam(max_norm=nan), adam(num=-1), adam(num=1 << 41), adam(null=None),
+              adam(m=None), adam(v=None), adam(state_bits=8), adam(workspace=None), adam(workspace=8), adam(workspace_bytes=64),
+              lib.apx_adamw_moments(one, one, one, one, 255, one, one, None), lib.apx_adamw_moments(one, one, one, one, -256, one, one, None), lib.apx_adamw_moments(None, one, one, one, 256, one, one, None)]
+    assert calls == [-1] * len(calls), [i for i, c in enumerate(calls) if c != -1]
+    assert b"invalid argument" in lib.apx_last_error()
+    assert lib.apx_gated_scan_save_floats(17, 2, 5) == 20 and lib.apx_gated_scan_save_floats(0, 2, 5) == 0
+    assert lib.apx_adamw_state_elements(3, (C.c_int64 * 3)(1, 0, 257)) == 768
+
+
+def test_wrappers_need_device_tensors():
+    from apex_amd import _lib, engine
+    f = torch.zeros(4, 2, 3)
+    for call in (lambda: engine.gated_scan(f, f), lambda: engine.gated_scan_backward(f, f, f, f), lambda: engine.gated_scan_step(f[0], f[0], f[0].clone()), lambda: engine.AdamW([f])):
+        with pytest.raises(_lib.ApxError):
+            call()
+
+
+def test_the_moments_noise_is_spread_evenly():
+    """Each of the 32 bits that round the moments is set for half of the elements, and neighbours, steps and seeds do not go together: 2^16 samples, five standard deviations."""
+    from oracle import sequence as Q
+    n = 1 << 16
+    a, b, c = Q.noise(7, 1, np.arange(n)), Q.noise(7, 2, np.arange(n)), Q.noise(8, 1, np.arange(n))
+    bits = lambda r: (r[:, None] >> np.arange(32, dtype=np.uint64)) & np.uint64(1)  # noqa: E731
+    lim = 5 * 0.5 / np.sqrt(n)
+    for r in (a, a ^ b, a ^ c, a[1:] ^ a[:-1], a[256:] ^ a[:-256]):
+        assert np.abs(bits(r).mean(0) - 0.5).max() < lim * 1.01

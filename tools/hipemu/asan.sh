@@ -18,7 +18,7 @@ else
 fi
 mkdir -p _build/$SAN
 FLAGS="-x c++ -std=c++17 -O1 -g -fPIC -pthread $SANFLAGS -I. -I../../apex_amd/csrc -I../../include -Wno-unused-function -Wno-unused-variable -Wno-unknown-attributes -Wno-ignored-attributes ${SWITCH:--DHIPEMU_STACK_MB=8}"
-for f in emul_ppo_small emul_learner emul_td3_small emul_env; do $CXX $FLAGS -c $f.cpp -o _build/$SAN/$f.o 2> /dev/null & done
+for f in emul_ppo_small emul_learner emul_td3_small emul_gated_scan emul_adamw emul_env; do $CXX $FLAGS -c $f.cpp -o _build/$SAN/$f.o 2> /dev/null & done
 wait
 $CXX -shared -pthread $LINKFLAGS _build/$SAN/*.o -ldl -o _build/libapx_emul_$SAN.so
 cd ../..

@@ -16,11 +16,12 @@ if [ "${1:-}" = check ]; then         # the env kernels' range-checked accessors
 fi
 pids=()
 grep -q ' fma ' /proc/cpuinfo && FLAGS="$FLAGS -mfma"      # fmaf as one instruction where the host has it (the env kernels' lane operations are fused multiply-adds)
-for u in emul_ppo_small emul_learner emul_td3_small emul_env; do
+for u in emul_ppo_small emul_learner emul_td3_small emul_gated_scan emul_adamw emul_env; do
     EX=; [ $u = emul_env ] && EX="${ENVFLAGS:-}"
+    [ $u = emul_adamw ] && EX=-ffp-contract=off      # (as in the product's Makefile)
     $CXX $FLAGS $EX -c $u.cpp -o $OBJ/$u.o &
     pids+=($!)
 done
 for p in "${pids[@]}"; do wait "$p"; done      # (set -e: a failed translation unit ends the script here)
-$CXX -shared -pthread $OBJ/emul_ppo_small.o $OBJ/emul_learner.o $OBJ/emul_td3_small.o $OBJ/emul_env.o -ldl -o _build/$OUT
+$CXX -shared -pthread $OBJ/emul_ppo_small.o $OBJ/emul_learner.o $OBJ/emul_td3_small.o $OBJ/emul_gated_scan.o $OBJ/emul_adamw.o $OBJ/emul_env.o -ldl -o _build/$OUT
 echo built tools/hipemu/_build/$OUT
