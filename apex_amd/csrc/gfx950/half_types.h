@@ -14,4 +14,7 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }        // v_rcp_f32: 1 ulp
 __device__ __forceinline__ float sqrt_fast(float x) { return __builtin_amdgcn_sqrtf(x); }      // v_sqrt_f32: 1 ulp
 
+// the value of the first lane, for what is the same in all lanes of a wave (a scalar register then)
+__device__ __forceinline__ int wave_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 }  // namespace half_types

@@ -34,4 +34,6 @@ inline float exp2_fast(float x) { return exp2f(x); }
 inline float rcp_fast(float x) { return 1.0f / x; }
 inline float sqrt_fast(float x) { return sqrtf(x); }
 
+inline int wave_uniform(int x) { return x; }
+
 }  // namespace half_types
