@@ -133,7 +133,7 @@ SIGNATURES = {
     "apx_gated_scan_backward": (C.c_int, [C.POINTER(GatedScanArgs), c_ptr]),
     "apx_gated_scan_step": (C.c_int, [C.POINTER(GatedScanArgs), c_ptr, c_ptr]),
     "apx_adamw_state_elements": (C.c_int64, [C.c_int, c_ptr]),
-    "apx_adamw_workspace_bytes": (C.c_size_t, [C.c_int]),
+    "apx_adamw_workspace_bytes": (C.c_size_t, [C.c_int, c_ptr]),
     "apx_adamw": (C.c_int, [C.POINTER(AdamwArgs), c_ptr]),
     "apx_adamw_moments": (C.c_int, [c_ptr, c_ptr, c_ptr, c_ptr, C.c_int64, c_ptr, c_ptr, c_ptr]),
     "apx_env_default_cfg": (None, [C.POINTER(EnvCfg)]),

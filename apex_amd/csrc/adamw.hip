@@ -14,35 +14,55 @@ namespace {
 
 using namespace half_types;
 
-constexpr int TABLE = 90;                  // tensors a launch: 40 bytes each, of 4 kB of kernel arguments
+constexpr int TABLE = 120;                 // entries a launch: 32 bytes each, of 4 kB of kernel arguments
 constexpr int BLOCK = 256;                 // elements that share a scale of 8-bit moments, and what a tensor's part of the moments is rounded up to
-constexpr int CHUNK = 2048;                // elements a workgroup takes at a time: 8 blocks
+constexpr int CHUNK = 2048;                // elements a workgroup takes at a time: 8 blocks, 8 elements a thread
+constexpr int64_t ENTRY = (int64_t)1 << 31;      // elements of an entry: a larger tensor takes several
 constexpr int PARTS = 1024;                // partial sums of squares of one launch
 constexpr int GRID = 2048;                 // workgroups of the update at most: 8 for each of 256 CUs
 constexpr unsigned M_OFFSET = 904, V_OFFSET = 776;
 
 struct Table {
-    float* p[TABLE]; const void* g[TABLE]; int64_t n[TABLE];
-    int64_t state[TABLE];                  // where the tensor's moments begin
+    float* p[TABLE]; const void* g[TABLE];
+    unsigned n[TABLE], state[TABLE];       // elements; the block its moments begin with
     int first[TABLE];                      // its first chunk
     float wd[TABLE];
-    int tensors, chunks;
+    int entries, chunks;
 };
 struct Step { float step, ibc; };
 
-// the tensor of a chunk: the last whose first chunk is not beyond it (empty tensors share a first chunk with the next one and are passed over)
-__device__ __forceinline__ int tensor_of(const Table& T, int chunk) {
-    int lo = 0, hi = T.tensors - 1;
+// the entry of a chunk: the last whose first chunk is not beyond it
+__device__ __forceinline__ int entry_of(const Table& T, int chunk) {
+    int lo = 0, hi = T.entries - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (T.first[mid] <= chunk) lo = mid; else hi = mid - 1;
     }
     return lo;
 }
+// 4 elements by one wide access, on any boundary that their type allows (tensors are views at any offset of a flat block)
+struct alignas(4) F4 { float v[4]; };
+struct alignas(2) H4 { uint16_t v[4]; };
+template <int TYPE> __device__ __forceinline__ void load_grad(const void* g, int64_t i, float (&o)[4]) {
+    if constexpr (TYPE == APX_F32) {
+        const F4 r = *(const F4*)((const float*)g + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = r.v[k];
+    } else {
+        const H4 r = *(const H4*)((const uint16_t*)g + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = TYPE == APX_BF16 ? widen_bf16(r.v[k]) : widen_f16(r.v[k]);
+    }
+}
 template <int TYPE> __device__ __forceinline__ float grad_at(const void* g, int64_t i) {
     if constexpr (TYPE == APX_F32) return ((const float*)g)[i];
     else if constexpr (TYPE == APX_BF16) return widen_bf16(((const uint16_t*)g)[i]);
     else return widen_f16(((const uint16_t*)g)[i]);
+}
+// up to 4 elements at i of which `have` exist; the others are 0
+template <int TYPE> __device__ __forceinline__ void load_grad_end(const void* g, int64_t i, int have, float (&o)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = k < have ? grad_at<TYPE>(g, i + k) : 0.f;
 }
 // sum over the workgroup's 256 threads in a fixed order; every thread gets it
 __device__ __forceinline__ double block_sum(double v) {
@@ -70,14 +90,14 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(Table T, double* parts,
     if (t && blockIdx.x == 0 && threadIdx.x == 0) count_step(t, out, lr, beta1, beta2);
     double sum = 0;
     for (int chunk = blockIdx.x; chunk < T.chunks; chunk += gridDim.x) {
-        const int k = tensor_of(T, chunk);
-        const int64_t e0 = (int64_t)(chunk - T.first[k]) * CHUNK;
-        const int64_t left = T.n[k] - e0;
-        const int n = left < CHUNK ? (int)left : CHUNK;
-        for (int i = threadIdx.x; i < n; i += 256) {
-            const double g = (double)grad_at<TYPE>(T.g[k], e0 + i);
-            sum += g * g;
-        }
+        const int k = entry_of(T, chunk);
+        const unsigned e0 = (unsigned)(chunk - T.first[k]) * CHUNK, left = T.n[k] - e0, i = threadIdx.x * 4;
+        const void* p = T.g[k];
+        float g[2][4];
+        if (left >= CHUNK) { load_grad<TYPE>(p, (int64_t)e0 + i, g[0]); load_grad<TYPE>(p, (int64_t)e0 + 1024 + i, g[1]); }
+        else { load_grad_end<TYPE>(p, (int64_t)e0 + i, (int)left - (int)i, g[0]); load_grad_end<TYPE>(p, (int64_t)e0 + 1024 + i, (int)left - 1024 - (int)i, g[1]); }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) sum += (double)g[q >> 2][q & 3] * (double)g[q >> 2][q & 3];
     }
     sum = block_sum(sum);
     if (threadIdx.x == 0) parts[blockIdx.x] = sum;
@@ -109,17 +129,32 @@ __device__ __forceinline__ void adam(float g, float& m, float& v, float& p, cons
 
 template <int TYPE>
 __global__ __launch_bounds__(256) void adamw32_kernel(Table T, Hyper P, float* __restrict__ M, float* __restrict__ V) {
-    float k;
-    if (!clip_factor(P, blockIdx.x == 0, k)) return;
+    float c;      // what a gradient is multiplied by
+    if (!clip_factor(P, blockIdx.x == 0, c)) return;
     const Step S = *P.step;
     for (int chunk = blockIdx.x; chunk < T.chunks; chunk += gridDim.x) {
-        const int id = tensor_of(T, chunk);
-        const int64_t e0 = (int64_t)(chunk - T.first[id]) * CHUNK;
-        const int64_t left = T.n[id] - e0;
-        const int n = left < CHUNK ? (int)left : CHUNK;
-        float* p = T.p[id] + e0; float* m = M + T.state[id] + e0; float* v = V + T.state[id] + e0;
+        const int id = entry_of(T, chunk);
+        const unsigned e0 = (unsigned)(chunk - T.first[id]) * CHUNK, left = T.n[id] - e0;
+        float* p = T.p[id] + e0; float* m = M + (int64_t)T.state[id] * BLOCK + e0; float* v = V + (int64_t)T.state[id] * BLOCK + e0;
         const float keep = 1.f - P.lr * T.wd[id];
-        for (int i = threadIdx.x; i < n; i += 256) adam(grad_at<TYPE>(T.g[id], e0 + i) * k, m[i], v[i], p[i], P, S, keep);
+        if (left >= CHUNK) {
+            float g[2][4]; F4 pp[2], mm[2], vv[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int i = q * 1024 + threadIdx.x * 4;
+                load_grad<TYPE>(T.g[id], (int64_t)e0 + i, g[q]);
+                pp[q] = *(const F4*)(p + i); mm[q] = *(const F4*)(m + i); vv[q] = *(const F4*)(v + i);
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int i = q * 1024 + threadIdx.x * 4;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) adam(g[q][k] * c, mm[q].v[k], vv[q].v[k], pp[q].v[k], P, S, keep);
+                *(F4*)(p + i) = pp[q]; *(F4*)(m + i) = mm[q]; *(F4*)(v + i) = vv[q];
+            }
+        } else {
+            for (unsigned i = threadIdx.x; i < left; i += 256) adam(grad_at<TYPE>(T.g[id], (int64_t)e0 + i) * c, m[i], v[i], p[i], P, S, keep);
+        }
     }
 }
 
@@ -162,63 +197,108 @@ __device__ __forceinline__ float decode_m(unsigned c, float s) {
 }
 __device__ __forceinline__ float decode_v(unsigned c, float s) { return (c ? __uint_as_float((c + V_OFFSET) << 20) : 0.f) * s; }
 
-// a wave takes a block of 256 elements, a lane 4 of them
+// the largest of a wave's 64 numbers, as a scalar: four exchanges inside the rows of 16 lanes, then the rows' numbers as scalars
+__device__ __forceinline__ unsigned wave_top(unsigned x) {
+    auto top = [&](int y) { x = x > (unsigned)y ? x : (unsigned)y; };
+    top(__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, true));       // lanes 1 apart
+    top(__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));       // 2 apart
+    top(__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, true));      // the other half of 8
+    top(__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xF, 0xF, true));      // the other half of 16
+    unsigned r = (unsigned)__builtin_amdgcn_readlane((int)x, 0);
+#pragma unroll
+    for (int row = 16; row < 64; row += 16) { const unsigned y = (unsigned)__builtin_amdgcn_readlane((int)x, row); r = r > y ? r : y; }
+    return r;
+}
+struct alignas(4) Code4 { uint8_t v[4]; };
+
+// A wave takes a block of 256 elements at a time, a lane 4 of them, two blocks of a chunk at once so that twice as many loads are on their way.  Codes and scales are exact in
+// f32 (scales are powers of two), the block's largest is found on the bits, so the same inputs give the same codes whatever the launch looks like.
 template <int TYPE>
 __global__ __launch_bounds__(256) void adamw8_kernel(Table T, Hyper P, uint8_t* __restrict__ M, uint8_t* __restrict__ V, float* __restrict__ MS, float* __restrict__ VS) {
-    float k;
-    if (!clip_factor(P, blockIdx.x == 0, k)) return;
+    float c;      // what a gradient is multiplied by
+    if (!clip_factor(P, blockIdx.x == 0, c)) return;
     const Step S = *P.step;
     const unsigned key = step_key(P.seed, *P.t);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = wave_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     for (int chunk = blockIdx.x; chunk < T.chunks; chunk += gridDim.x) {
-        const int id = tensor_of(T, chunk);
+        const int id = entry_of(T, chunk);
         const float keep = 1.f - P.lr * T.wd[id];
-        for (int q = wave; q < CHUNK / BLOCK; q += 4) {
-            const int64_t e = (int64_t)(chunk - T.first[id]) * CHUNK + q * BLOCK;
-            if (e >= T.n[id]) break;
-            const int64_t at = T.state[id] + e, blk = at / BLOCK;
-            const float ms = MS[blk], vs = VS[blk];
-            float* p = T.p[id];
+        const unsigned n = T.n[id], e0 = (unsigned)(chunk - T.first[id]) * CHUNK;
+        float* const p = T.p[id];
+        float g[2][4], ms[2], vs[2]; F4 pp[2]; Code4 mm[2], vv[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const unsigned e = e0 + (q * 4 + wave) * BLOCK;
+            if (e >= n) continue;
+            const int64_t blk = (int64_t)T.state[id] + e / BLOCK;
+            const unsigned i = e + lane * 4;
+            if (n - e >= BLOCK) { load_grad<TYPE>(T.g[id], i, g[q]); pp[q] = *(const F4*)(p + i); }
+            else {
+                load_grad_end<TYPE>(T.g[id], i, (int)(n - e) - lane * 4, g[q]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) pp[q].v[k] = i + k < n ? p[i + k] : 0.f;
+            }
+            mm[q] = *(const Code4*)(M + blk * BLOCK + lane * 4); vv[q] = *(const Code4*)(V + blk * BLOCK + lane * 4);
+            ms[q] = MS[blk]; vs[q] = VS[blk];
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const unsigned e = e0 + (q * 4 + wave) * BLOCK;
+            if (e >= n) continue;
+            const int64_t blk = (int64_t)T.state[id] + e / BLOCK;
+            const unsigned i = e + lane * 4;
             float m[4], v[4];
             unsigned mt = 0, vt = 0;
-            for (int i = 0; i < 4; ++i) {
-                const int64_t j = e + lane * 4 + i;
-                m[i] = v[i] = 0.f;
-                if (j < T.n[id]) {
-                    m[i] = decode_m(M[at + lane * 4 + i], ms); v[i] = decode_v(V[at + lane * 4 + i], vs);
-                    adam(grad_at<TYPE>(T.g[id], j) * k, m[i], v[i], p[j], P, S, keep);
-                }
-                const unsigned am = __float_as_uint(m[i]) & 0x7fffffffu, av = __float_as_uint(v[i]) & 0x7fffffffu;      // (as integers: a NaN is larger than all numbers)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {      // (behind the tensor's end: codes, gradient and parameter 0 stay 0)
+                m[k] = decode_m(mm[q].v[k], ms[q]); v[k] = decode_v(vv[q].v[k], vs[q]);
+                adam(g[q][k] * c, m[k], v[k], pp[q].v[k], P, S, keep);
+                if (n - e < BLOCK && i + k >= n) m[k] = v[k] = 0.f;      // (0 times an infinite scale factor, say)
+                const unsigned am = __float_as_uint(m[k]) & 0x7fffffffu, av = __float_as_uint(v[k]) & 0x7fffffffu;      // (as integers: a NaN is larger than all numbers)
                 mt = mt > am ? mt : am; vt = vt > av ? vt : av;
             }
+            if (n - e >= BLOCK) *(F4*)(p + i) = pp[q];
+            else {
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                const unsigned a = __shfl_xor(mt, o, 64), b = __shfl_xor(vt, o, 64);
-                mt = mt > a ? mt : a; vt = vt > b ? vt : b;
+                for (int k = 0; k < 4; ++k) if (i + k < n) p[i + k] = pp[q].v[k];
             }
             float s, inv, s2, inv2;
-            block_scale(mt, s, inv); block_scale(vt, s2, inv2);
-            for (int i = 0; i < 4; ++i) {
-                const int64_t j = at + lane * 4 + i;
-                const unsigned r = element_noise(key, j);
-                M[j] = (uint8_t)encode_m(m[i], inv, r & 0xffffu);
-                V[j] = (uint8_t)encode_v(v[i], inv2, r >> 16);
+            block_scale(wave_top(mt), s, inv); block_scale(wave_top(vt), s2, inv2);
+            Code4 mo, vo;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const unsigned r = element_noise(key, blk * BLOCK + lane * 4 + k);
+                mo.v[k] = (uint8_t)encode_m(m[k], inv, r & 0xffffu); vo.v[k] = (uint8_t)encode_v(v[k], inv2, r >> 16);
             }
+            *(Code4*)(M + blk * BLOCK + lane * 4) = mo; *(Code4*)(V + blk * BLOCK + lane * 4) = vo;
             if (lane == 0) { MS[blk] = s; VS[blk] = s2; }
         }
     }
 }
 
+struct alignas(16) Half8 { uint16_t v[8]; };
+struct alignas(8) Code8 { uint8_t v[8]; };
+// 8 elements a thread: blocks of 256 are whole, and the moments' own buffers are aligned
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const uint8_t* __restrict__ M, const uint8_t* __restrict__ V, const float* __restrict__ MS, const float* __restrict__ VS,
                                                             int64_t n, uint16_t* __restrict__ mo, uint16_t* __restrict__ vo) {
-    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        mo[i] = round_bf16(decode_m(M[i], MS[i / BLOCK])); vo[i] = round_bf16(decode_v(V[i], VS[i / BLOCK]));
+    for (int64_t i = (blockIdx.x * (int64_t)256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
+        const Code8 m = *(const Code8*)(M + i), v = *(const Code8*)(V + i);
+        const float ms = MS[i / BLOCK], vs = VS[i / BLOCK];
+        Half8 a, b;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { a.v[k] = round_bf16(decode_m(m.v[k], ms)); b.v[k] = round_bf16(decode_v(v.v[k], vs)); }
+        *(Half8*)(mo + i) = a; *(Half8*)(vo + i) = b;
     }
 }
 
 struct Workspace { Step* step; double* parts; };
 Workspace workspace_of(void* w) { return {(Step*)w, (double*)((char*)w + 64)}; }
-int launches_of(int n_tensors) { return (n_tensors + TABLE - 1) / TABLE; }
+int64_t entries_of(int n_tensors, const int64_t* numel) {
+    int64_t k = 0;
+    for (int i = 0; i < n_tensors; ++i) k += numel[i] > 0 ? (numel[i] + ENTRY - 1) / ENTRY : 0;
+    return k;
+}
+int launches_of(int n_tensors, const int64_t* numel) { return (int)((entries_of(n_tensors, numel) + TABLE - 1) / TABLE); }
 
 }  // namespace
 
@@ -235,7 +315,7 @@ extern "C" int64_t apx_adamw_state_elements(int n_tensors, const int64_t* numel)
     for (int i = 0; i < n_tensors; ++i) n += numel[i] > 0 ? (numel[i] + BLOCK - 1) / BLOCK * BLOCK : 0;
     return n;
 }
-extern "C" size_t apx_adamw_workspace_bytes(int n_tensors) { return n_tensors > 0 ? 64 + (size_t)launches_of(n_tensors) * PARTS * sizeof(double) : 0; }
+extern "C" size_t apx_adamw_workspace_bytes(int n_tensors, const int64_t* numel) { return 64 + (size_t)launches_of(n_tensors, numel) * PARTS * sizeof(double); }
 
 extern "C" int apx_adamw(const apx_adamw_args* a, void* stream) {
     APX_REQUIRE(a && a->n_tensors >= 0, "args");
@@ -247,36 +327,45 @@ extern "C" int apx_adamw(const apx_adamw_args* a, void* stream) {
     APX_REQUIRE((float)a->eps >= 1.17549435e-38f && std::isfinite((float)a->eps) && std::isfinite((float)a->lr) && std::isfinite((float)a->grad_scale) && !std::isnan(a->max_norm), "eps, lr, grad_scale, max_norm");
     int64_t total = 0;
     for (int i = 0; i < a->n_tensors; ++i) {
-        APX_REQUIRE(a->numel[i] >= 0 && a->numel[i] < ((int64_t)1 << 40), "numel");
+        APX_REQUIRE(a->numel[i] >= 0 && a->numel[i] < ((int64_t)1 << 39), "numel");
         APX_REQUIRE(a->numel[i] == 0 || (a->params[i] && a->grads[i]), "null tensor");
         total += a->numel[i];
     }
-    APX_REQUIRE(total < ((int64_t)1 << 41), "numel in all");
+    APX_REQUIRE(total < ((int64_t)1 << 39), "numel in all");
     APX_REQUIRE(total == 0 || (a->m && a->v && (a->state_bits == 32 || (a->m_scale && a->v_scale))), "moments");
-    APX_REQUIRE(a->workspace && ((uintptr_t)a->workspace & 15) == 0 && a->workspace_bytes >= apx_adamw_workspace_bytes(a->n_tensors), "workspace");
+    APX_REQUIRE((((uintptr_t)a->m | (uintptr_t)a->v | (uintptr_t)a->m_scale | (uintptr_t)a->v_scale) & 3) == 0, "moments: 4-byte alignment");
+    APX_REQUIRE(a->workspace && ((uintptr_t)a->workspace & 15) == 0 && a->workspace_bytes >= apx_adamw_workspace_bytes(a->n_tensors, a->numel), "workspace");
     const hipStream_t s = (hipStream_t)stream;
     const Workspace W = workspace_of(a->workspace);
     const bool clip = a->max_norm > 0;
-    const int n_launches = launches_of(a->n_tensors);
-    auto table = [&](int l, int64_t& state) {
-        Table T;
-        T.tensors = 0; T.chunks = 0;
-        for (int i = l * TABLE; i < a->n_tensors && i < (l + 1) * TABLE; ++i) {
-            const int k = T.tensors++;
-            T.p[k] = a->params[i]; T.g[k] = a->grads[i]; T.n[k] = a->numel[i]; T.state[k] = state; T.first[k] = T.chunks;
-            T.wd[k] = a->weight_decay ? a->weight_decay[i] : 0.f;
-            T.chunks += (int)((a->numel[i] + CHUNK - 1) / CHUNK);
-            state += (a->numel[i] + BLOCK - 1) / BLOCK * BLOCK;
+    // the entries in order, a launch's worth at a time
+    struct Walk { int tensor; int64_t done, state; };
+    auto next = [&](Walk& w, Table& T) {
+        T.entries = T.chunks = 0;
+        while (w.tensor < a->n_tensors && T.entries < TABLE) {
+            const int i = w.tensor;
+            const int64_t left = a->numel[i] - w.done, n = left < ENTRY ? left : ENTRY;
+            if (n > 0) {
+                const int k = T.entries++;
+                T.p[k] = a->params[i] + w.done;
+                T.g[k] = (const char*)a->grads[i] + w.done * (a->grad_type == APX_F32 ? 4 : 2);
+                T.n[k] = (unsigned)n; T.state[k] = (unsigned)w.state; T.first[k] = T.chunks;
+                T.wd[k] = a->weight_decay ? a->weight_decay[i] : 0.f;
+                T.chunks += (int)((n + CHUNK - 1) / CHUNK);
+                w.state += (n + BLOCK - 1) / BLOCK;
+                w.done += n;
+            }
+            if (w.done == a->numel[i]) { ++w.tensor; w.done = 0; }
         }
-        return T;
+        return T.entries > 0;
     };
+    Table T;
     int n_parts = 0;
     if (clip) {
-        int64_t state = 0;
-        for (int l = 0; l < n_launches; ++l) {
-            const Table T = table(l, state);
+        Walk w = {0, 0, 0};
+        for (bool first = true; next(w, T) || first; first = false) {
             const int grid = T.chunks < 1 ? 1 : T.chunks < PARTS ? T.chunks : PARTS;
-            APX_BY_TYPE(a->grad_type, adamw_norm_kernel, grid, 256, s, T, W.parts + n_parts, l == 0 ? a->t : (int64_t*)nullptr, W.step, a->lr, a->beta1, a->beta2);
+            APX_BY_TYPE(a->grad_type, adamw_norm_kernel, grid, 256, s, T, W.parts + n_parts, first ? a->t : (int64_t*)nullptr, W.step, a->lr, a->beta1, a->beta2);
             n_parts += grid;
         }
     } else {
@@ -285,13 +374,11 @@ extern "C" int apx_adamw(const apx_adamw_args* a, void* stream) {
     }
     const Hyper P = {(float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps, (float)a->lr, (float)a->grad_scale, (float)a->max_norm,
                      W.parts, n_parts, W.step, a->t, a->seed, a->norm_out};
-    int64_t state = 0;
-    for (int l = 0; l < n_launches; ++l) {
-        const Table T = table(l, state);
-        if (T.chunks == 0 && l > 0) continue;
+    Walk w = {0, 0, 0};
+    for (bool first = true; next(w, T) || first; first = false) {      // (a set of empty tensors counts a step and has a norm of 0)
         const int grid = T.chunks < 1 ? 1 : T.chunks < GRID ? T.chunks : GRID;
         Hyper Q = P;
-        if (l > 0) Q.norm_out = nullptr;
+        if (!first) Q.norm_out = nullptr;
         if (a->state_bits == 32) APX_BY_TYPE(a->grad_type, adamw32_kernel, grid, 256, s, T, Q, (float*)a->m, (float*)a->v);
         else APX_BY_TYPE(a->grad_type, adamw8_kernel, grid, 256, s, T, Q, (uint8_t*)a->m, (uint8_t*)a->v, a->m_scale, a->v_scale);
     }
@@ -302,7 +389,8 @@ extern "C" int apx_adamw_moments(const void* m, const void* v, const float* m_sc
     APX_REQUIRE(elements >= 0 && elements % BLOCK == 0, "elements: whole blocks of 256");
     if (elements == 0) return APX_OK;
     APX_REQUIRE(m && v && m_scale && v_scale && m_out && v_out, "null pointer");
-    const int64_t want = (elements + 255) / 256;
+    APX_REQUIRE((((uintptr_t)m | (uintptr_t)v) & 7) == 0 && (((uintptr_t)m_out | (uintptr_t)v_out) & 15) == 0, "alignment");
+    const int64_t want = (elements + 2047) / 2048;
     hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)(want < GRID ? want : GRID)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)m, (const uint8_t*)v, m_scale, v_scale,
                        elements, (uint16_t*)m_out, (uint16_t*)v_out);
     APX_LAUNCH_CHECK();

@@ -1,7 +1,8 @@
 """Tensor-level wrappers over the C ABI (include/apx.h).  PyTorch-ROCm is plumbing here: device memory, streams,
 torch.distributed.  Every function launches HIP kernels from libapx.so on the current torch stream."""
+import array
 import ctypes as C
-import functools
+import struct
 
 import numpy as np
 import torch
@@ -202,127 +203,122 @@ class Lstm:
 
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # APX_F32, APX_BF16, APX_F16
+_SCAN_ARGS = struct.Struct("2i35q")      # apx_gated_scan_args: packed in one go (field by field it was 10 us a call, three times a step's kernel)
 
 
-def _on_device_of(fn):
-    """Run fn with its first tensor's device as the current one: the stream and the workspaces of the call are that device's."""
-    @functools.wraps(fn)
-    def call(*a, **k):
-        t = next((v for v in (*a, *k.values()) if torch.is_tensor(v)), None)
-        if t is None or not t.is_cuda or t.device.index == torch.cuda.current_device():
-            return fn(*a, **k)
-        with torch.cuda.device(t.device):
-            return fn(*a, **k)
-    return call
+def _elsewhere(fn, dev, *a, **k):
+    """fn with device `dev` as the current one: the stream and the workspaces of the call are that device's."""
+    with torch.cuda.device(dev):
+        return fn(*a, **k)
 
 
-def _seq_in(name, t, shape, like):
-    """An operand [.., H] of the sequence operators as they take it: same shape, type and device, the units of a row next to each other."""
-    if t.shape != shape or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError("%s is %s %s on %s, expected %s %s on %s" % (name, tuple(t.shape), t.dtype, t.device, tuple(shape), like.dtype, like.device))
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+def _operand(name, t, like, dev, out=False):
+    """(t, its three numbers in apx_gated_scan_args) for an operand [.., H] of f's shape, type and device; one whose units do not lie next to each other is copied (an output refused)"""
+    if t.shape != like.shape or t.dtype != like.dtype or t.get_device() != dev:
+        raise ValueError("%s is %s %s on %s, expected %s %s on %s" % (name, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype, like.device))
+    s = t.stride()
+    if s[-1] != 1 and t.shape[-1] > 1:
+        if out:
+            raise ValueError("%s has stride %d along the units, expected 1" % (name, s[-1]))
+        t = t.contiguous(); s = t.stride()
+    return t, (t.data_ptr(), s[0] if len(s) == 3 else 0, s[-2])
 
 
-def _seq_out(name, t, shape, like):
+def _extra(name, t, shape, dtype, like, dev):
+    """t as a dense tensor of that shape and type, and its pointer"""
     if t is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    if t.shape != shape or t.dtype != like.dtype or t.device != like.device or (t.stride(-1) != 1 and t.shape[-1] > 1):
-        raise ValueError("%s is %s %s on %s, expected %s %s on %s with stride 1 along the units" % (name, tuple(t.shape), t.dtype, t.device, tuple(shape), like.dtype, like.device))
-    return t
+        return None, 0
+    if tuple(t.shape) != shape or t.dtype != dtype or t.get_device() != dev:
+        raise ValueError("%s is %s %s on %s, expected %s %s on %s" % (name, tuple(t.shape), t.dtype, t.device, shape, dtype, like.device))
+    t = t.contiguous()
+    return t, t.data_ptr()
 
 
-def _state(name, t, B, H, device):
-    if t is None:
-        return None
-    if tuple(t.shape) != (B, H) or t.dtype != torch.float32 or t.device != device:
-        raise ValueError("%s is %s %s on %s, expected [%d, %d] f32 on %s" % (name, tuple(t.shape), t.dtype, t.device, B, H, device))
-    return t.contiguous()
+_NONE = (0, 0, 0)
 
 
-def _rows(name, t, shape, dtype, device):
-    if t is None:
-        return None
-    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device:
-        raise ValueError("%s is %s %s on %s, expected %s %s on %s" % (name, tuple(t.shape), t.dtype, t.device, shape, dtype, device))
-    return t.contiguous()
-
-
-def _gated_scan_args(f, x, o, h0, reset, lens):
+def _scan_inputs(f, x, o, h0, reset, lens, dim=3):
     _need_gpu(f, x, o, h0, reset, lens)
-    if f.dim() != 3 or f.dtype not in _TYPES:
-        raise ValueError("f is %s %s, expected [T, B, H] in f32, bf16 or f16" % (tuple(f.shape), f.dtype))
-    T, B, H = f.shape
-    f = _seq_in("f", f, f.shape, f); x = _seq_in("x", x, f.shape, f); o = None if o is None else _seq_in("o", o, f.shape, f)
-    h0 = _state("h0", h0, B, H, f.device); reset = _rows("reset", reset, (T, B), torch.uint8, f.device); lens = _rows("lens", lens, (B,), torch.int32, f.device)
-    a = _lib.GatedScanArgs(type=_TYPES[f.dtype], H=H, T=T, B=B, f=_p(f), f_t=f.stride(0), f_b=f.stride(1), x=_p(x), x_t=x.stride(0), x_b=x.stride(1), h0=_p(h0), reset=_p(reset),
-                           lens=_p(lens))
-    if o is not None:
-        a.o, a.o_t, a.o_b = _p(o), o.stride(0), o.stride(1)
-    need = int(_lib.load().apx_gated_scan_workspace_bytes(T, B, H))
-    ws = torch.empty(need, dtype=torch.uint8, device=f.device) if need else None      # of this call alone: calls on two streams, and two captured graphs, never share it
-    a.workspace, a.workspace_bytes = _p(ws), need
-    return a, (f, x, o, h0, reset, lens, ws)      # (the tensors the arguments point into)
+    if f.dim() != dim or f.dtype not in _TYPES:
+        raise ValueError("f is %s %s, expected [%sB, H] in f32, bf16 or f16" % (tuple(f.shape), f.dtype, "T, " if dim == 3 else ""))
+    dev = f.get_device()
+    B, H = f.shape[-2:]
+    lead = tuple(f.shape[:-1])
+    f, f3 = _operand("f", f, f, dev); x, x3 = _operand("x", x, f, dev); o, o3 = _operand("o", o, f, dev) if o is not None else (None, _NONE)
+    h0, h0p = _extra("h0", h0, (B, H), torch.float32, f, dev)
+    reset, rp = _extra("reset", reset, lead, torch.uint8, f, dev)
+    lens, lp = _extra("lens", lens, (B,), torch.int32, f, dev)
+    head = (_TYPES[f.dtype], H, f.shape[0] if dim == 3 else 1, B, *f3, *x3, *o3, h0p, rp, lp)
+    return head, dev, (f, x, o, h0, reset, lens)      # (the tensors that the numbers point into)
 
 
-@_on_device_of
+def _scan_workspace(lib, T, B, H, like):
+    need = lib.apx_gated_scan_workspace_bytes(T, B, H)
+    if not need:
+        return None, 0, 0
+    ws = torch.empty(need, dtype=torch.uint8, device=like.device)      # of this call alone: calls on two streams, and two captured graphs, never share it
+    return ws, ws.data_ptr(), need
+
+
 def gated_scan(f, x, o=None, h0=None, reset=None, lens=None, keep=False, out=None):
     """The gated linear recurrence h_t = sigmoid(f_t) h_{t-1} + sigmoid(-f_t) x_t over [T, B, H] (f32, bf16 or f16; any strides with the units of a row next to each other, so
     slices of one product's rows need no copy).  y = h, or h sigmoid(o).  h0 [B, H] f32 = the carried state (None: zero); reset [T, B] uint8: a non-zero byte starts that step
     from a zero state (an episode start); lens [B] int32: steps from lens[b] on are padding - the state stays and y is 0 there.  out: where y goes (it must not lie on an input).
     Returns (y [T, B, H], h_last [B, H] f32), with keep=True (y, h_last, save) for gated_scan_backward.  States, gates and sums are f32 whatever the type."""
-    a, held = _gated_scan_args(f, x, o, h0, reset, lens)
+    head, dev, held = _scan_inputs(f, x, o, h0, reset, lens)
+    if dev >= 0 and dev != torch.cuda.current_device():
+        return _elsewhere(gated_scan, dev, f, x, o, h0, reset, lens, keep, out)
     lib = _lib.load()
-    y = _seq_out("out", out, f.shape, f)
-    h_last = torch.empty(a.B, a.H, dtype=torch.float32, device=f.device)
-    save = torch.empty(int(lib.apx_gated_scan_save_floats(a.T, a.B, a.H)), dtype=torch.float32, device=f.device) if keep else None
-    a.y, a.y_t, a.y_b, a.h_last, a.save = _p(y), y.stride(0), y.stride(1), _p(h_last), _p(save)
+    _, H, T, B = head[:4]
+    y, y3 = _operand("out", torch.empty(f.shape, dtype=f.dtype, device=f.device) if out is None else out, f, dev, True)
+    h_last = torch.empty(B, H, dtype=torch.float32, device=f.device)
+    save = torch.empty(lib.apx_gated_scan_save_floats(T, B, H), dtype=torch.float32, device=f.device) if keep else None
+    ws, wp, wn = _scan_workspace(lib, T, B, H, f)
+    a = _lib.GatedScanArgs.from_buffer_copy(_SCAN_ARGS.pack(*head, *y3, h_last.data_ptr(), save.data_ptr() if keep else 0, *_NONE, 0, *_NONE, *_NONE, *_NONE, 0, wp, wn))
     check(lib.apx_gated_scan_forward(C.byref(a), _stream()))
     return (y, h_last, save) if keep else (y, h_last)
 
 
-@_on_device_of
 def gated_scan_backward(f, x, dy, save, o=None, h0=None, reset=None, lens=None, dh_last=None, out=None):
     """Gradients of gated_scan(f, x, o, h0, reset, lens, keep=True) for dy [T, B, H] and dh_last [B, H] f32 (None: 0): (df, dx, do, dh0), do None without o, dh0 f32 and None
     without h0.  out: (df, dx) or (df, dx, do) to write into - slices of one gradient of the product that made f | x | o, for instance."""
-    a, held = _gated_scan_args(f, x, o, h0, reset, lens)
-    lib = _lib.load()
+    head, dev, held = _scan_inputs(f, x, o, h0, reset, lens)
     _need_gpu(dy, save, dh_last)
-    dy = _seq_in("dy", dy, f.shape, f)
-    n = int(lib.apx_gated_scan_save_floats(a.T, a.B, a.H))
-    if save.numel() != n or save.dtype != torch.float32 or save.device != f.device or not save.is_contiguous():
+    if dev >= 0 and dev != torch.cuda.current_device():
+        return _elsewhere(gated_scan_backward, dev, f, x, dy, save, o, h0, reset, lens, dh_last, out)
+    lib = _lib.load()
+    _, H, T, B = head[:4]
+    dy, dy3 = _operand("dy", dy, f, dev)
+    n = lib.apx_gated_scan_save_floats(T, B, H)
+    if save.numel() != n or save.dtype != torch.float32 or save.get_device() != dev or not save.is_contiguous():
         raise ValueError("save has %d entries, gated_scan(keep=True) on these inputs makes %d" % (save.numel(), n))
-    dh_last = _state("dh_last", dh_last, a.B, a.H, f.device)
-    if out is not None and len(out) != (2 if o is None else 3):
-        raise ValueError("out holds %d tensors, expected %d" % (len(out), 2 if o is None else 3))
-    given = list(out) if out is not None else [None] * 3
-    df, dx = (_seq_out(k, g, f.shape, f) for k, g in zip(("df", "dx"), given))
-    do = _seq_out("do", given[2], f.shape, f) if o is not None else None
-    dh0 = torch.empty(a.B, a.H, dtype=torch.float32, device=f.device) if h0 is not None else None
-    a.dy, a.dy_t, a.dy_b, a.dh_last, a.save = _p(dy), dy.stride(0), dy.stride(1), _p(dh_last), _p(save)
-    a.df, a.df_t, a.df_b, a.dx, a.dx_t, a.dx_b, a.dh0 = _p(df), df.stride(0), df.stride(1), _p(dx), dx.stride(0), dx.stride(1), _p(dh0)
-    if do is not None:
-        a.do_, a.do_t, a.do_b = _p(do), do.stride(0), do.stride(1)
+    dh_last, dhp = _extra("dh_last", dh_last, (B, H), torch.float32, f, dev)
+    k = 2 if o is None else 3
+    if out is None:
+        out = [torch.empty(f.shape, dtype=f.dtype, device=f.device) for _ in range(k)]
+    elif len(out) != k:
+        raise ValueError("out holds %d tensors, expected %d" % (len(out), k))
+    df, df3 = _operand("df", out[0], f, dev, True); dx, dx3 = _operand("dx", out[1], f, dev, True)
+    do, do3 = _operand("do", out[2], f, dev, True) if o is not None else (None, _NONE)
+    dh0 = torch.empty(B, H, dtype=torch.float32, device=f.device) if h0 is not None else None
+    ws, wp, wn = _scan_workspace(lib, T, B, H, f)
+    a = _lib.GatedScanArgs.from_buffer_copy(_SCAN_ARGS.pack(*head, *_NONE, 0, save.data_ptr(), *dy3, dhp, *df3, *dx3, *do3, dh0.data_ptr() if dh0 is not None else 0, wp, wn))
     check(lib.apx_gated_scan_backward(C.byref(a), _stream()))
     return df, dx, do, dh0
 
 
-@_on_device_of
 def gated_scan_step(f, x, h, o=None, reset=None, out=None):
     """One step of gated_scan for a rollout: f, x, o [B, H], the carried state h [B, H] f32 updated in place (rows whose reset byte, uint8 [B], is non-zero start from zero);
     returns y [B, H]."""
-    _need_gpu(f, x, h, o, reset)
-    if f.dim() != 2 or f.dtype not in _TYPES:
-        raise ValueError("f is %s %s, expected [B, H] in f32, bf16 or f16" % (tuple(f.shape), f.dtype))
-    B, H = f.shape
-    f = _seq_in("f", f, f.shape, f); x = _seq_in("x", x, f.shape, f); o = None if o is None else _seq_in("o", o, f.shape, f)
-    if tuple(h.shape) != (B, H) or h.dtype != torch.float32 or h.device != f.device or not h.is_contiguous():
-        raise ValueError("h is %s %s on %s, expected a dense [%d, %d] f32 on %s" % (tuple(h.shape), h.dtype, h.device, B, H, f.device))
-    reset = _rows("reset", reset, (B,), torch.uint8, f.device)
-    y = _seq_out("out", out, f.shape, f)
-    a = _lib.GatedScanArgs(type=_TYPES[f.dtype], H=H, B=B, f=_p(f), f_b=f.stride(0), x=_p(x), x_b=x.stride(0), reset=_p(reset), y=_p(y), y_b=y.stride(0))
-    if o is not None:
-        a.o, a.o_b = _p(o), o.stride(0)
-    check(_lib.load().apx_gated_scan_step(C.byref(a), _p(h), _stream()))
+    head, dev, held = _scan_inputs(f, x, o, None, reset, None, 2)
+    _need_gpu(h)
+    if dev >= 0 and dev != torch.cuda.current_device():
+        return _elsewhere(gated_scan_step, dev, f, x, h, o, reset, out)
+    if h.shape != f.shape or h.dtype != torch.float32 or h.get_device() != dev or not h.is_contiguous():
+        raise ValueError("h is %s %s on %s, expected a dense %s f32 on %s" % (tuple(h.shape), h.dtype, h.device, tuple(f.shape), f.device))
+    y, y3 = _operand("out", torch.empty(f.shape, dtype=f.dtype, device=f.device) if out is None else out, f, dev, True)
+    a = _lib.GatedScanArgs.from_buffer_copy(_SCAN_ARGS.pack(*head, *y3, 0, 0, *_NONE, 0, *_NONE, *_NONE, *_NONE, 0, 0, 0))
+    check(_lib.load().apx_gated_scan_step(C.byref(a), C.c_void_p(h.data_ptr()), _stream()))
     return y
 
 
@@ -358,33 +354,46 @@ class AdamW:
         self.elements = int(lib.apx_adamw_state_elements(n, self._numel))
         z = lambda k, d: torch.zeros(k, dtype=d, device=self.device)
         code = torch.float32 if state_bits == 32 else torch.uint8
-        self.m, self.v = z(self.elements, code), z(self.elements, code)
-        self.m_scale, self.v_scale = (z(self.elements // 256, torch.float32), z(self.elements // 256, torch.float32)) if state_bits == 8 else (None, None)
-        self.t = z(1, torch.int64)
-        self.norm = z(1, torch.float64)
-        self._ws = torch.empty(int(lib.apx_adamw_workspace_bytes(n)), dtype=torch.uint8, device=self.device)
+        self._m, self._v = z(self.elements, code), z(self.elements, code)
+        self._m_scale, self._v_scale = (z(self.elements // 256, torch.float32), z(self.elements // 256, torch.float32)) if state_bits == 8 else (None, None)
+        self._t, self._norm = z(1, torch.int64), z(1, torch.float64)
+        self._ws = torch.empty(int(lib.apx_adamw_workspace_bytes(n, self._numel)), dtype=torch.uint8, device=self.device)
+        self._index, self._shapes = self.params[0].get_device(), [p.shape for p in self.params]
+        self._held = [p.detach() for p in self.params]      # (keeps the memory that the pointers below name)
+        self._pointers = [p.data_ptr() for p in self.params]
+        self._ps = array.array("Q", self._pointers)
+        self._args = _lib.AdamwArgs(n_tensors=n, state_bits=state_bits, params=self._ps.buffer_info()[0], numel=C.addressof(self._numel), weight_decay=C.addressof(self._decay),
+                                    m=_p(self.m), v=_p(self.v), m_scale=_p(self.m_scale), v_scale=_p(self.v_scale), t=_p(self.t), workspace=_p(self._ws),
+                                    workspace_bytes=self._ws.numel(), norm_out=_p(self.norm))
+
+    # the state's own memory: read it, or load into it with copy_()
+    m = property(lambda self: self._m); v = property(lambda self: self._v)
+    m_scale = property(lambda self: self._m_scale); v_scale = property(lambda self: self._v_scale)
+    t = property(lambda self: self._t); norm = property(lambda self: self._norm)
 
     def step(self, grads, grad_scale=1.0, lr=None):
         """One step on `grads`: one dense tensor for each of params (all f32, all bf16 or all f16), multiplied by grad_scale first (1 / world size of a summed gradient)."""
-        n = len(self.params)
+        n, index = len(self.params), self._index
         if len(grads) != n:
             raise ValueError("%d gradients for %d tensors" % (len(grads), n))
         _need_gpu(*grads)
         kind = grads[0].dtype
         if kind not in _TYPES:
             raise ValueError("gradients in %s: f32, bf16 and f16 are served" % (kind,))
-        for i, (g, p) in enumerate(zip(grads, self.params)):
-            if g.dtype != kind or g.device != self.device or g.shape != p.shape or not g.is_contiguous() or not p.is_contiguous():
-                raise ValueError("grads[%d] is %s %s on %s, expected a dense %s %s on %s" % (i, tuple(g.shape), g.dtype, g.device, tuple(p.shape), kind, self.device))
-        if self.device.type == "cuda" and self.device.index != torch.cuda.current_device():
-            with torch.cuda.device(self.device):
-                return self.step(grads, grad_scale, lr)
-        at = C.c_void_p * n
-        ps, gs = at(*[p.data_ptr() for p in self.params]), at(*[g.data_ptr() for g in grads])
-        a = _lib.AdamwArgs(n_tensors=n, grad_type=_TYPES[kind], state_bits=self.state_bits, params=C.addressof(ps), grads=C.addressof(gs), numel=C.addressof(self._numel),
-                           weight_decay=C.addressof(self._decay), m=_p(self.m), v=_p(self.v), m_scale=_p(self.m_scale), v_scale=_p(self.v_scale), t=_p(self.t),
-                           lr=self.lr if lr is None else lr, beta1=self.betas[0], beta2=self.betas[1], eps=self.eps, grad_scale=grad_scale,
-                           max_norm=0.0 if self.max_norm is None else self.max_norm, seed=self.seed, workspace=_p(self._ws), workspace_bytes=self._ws.numel(), norm_out=_p(self.norm))
+        if ([g.shape for g in grads] != self._shapes or any([g.dtype != kind for g in grads]) or any([g.get_device() != index for g in grads])
+                or not all([g.is_contiguous() for g in grads])):
+            for i, (g, p) in enumerate(zip(grads, self.params)):
+                if g.dtype != kind or g.device != self.device or g.shape != p.shape or not g.is_contiguous():
+                    raise ValueError("grads[%d] is %s %s on %s, expected a dense %s %s on %s" % (i, tuple(g.shape), g.dtype, g.device, tuple(p.shape), kind, self.device))
+        at = [p.data_ptr() for p in self.params]
+        if at != self._pointers:
+            raise ValueError("a tensor of params has moved since this optimiser was made: it works on the memory that it was given")
+        if index >= 0 and index != torch.cuda.current_device():
+            return _elsewhere(self.step, index, grads, grad_scale, lr)
+        gs = array.array("Q", [g.data_ptr() for g in grads])
+        a = self._args
+        a.grad_type, a.grads, a.lr, a.grad_scale = _TYPES[kind], gs.buffer_info()[0], self.lr if lr is None else lr, grad_scale
+        a.beta1, a.beta2, a.eps, a.max_norm, a.seed = *self.betas, self.eps, 0.0 if self.max_norm is None else self.max_norm, self.seed
         check(_lib.load().apx_adamw(C.byref(a), _stream()))
 
     def moments(self):

@@ -282,8 +282,9 @@ int apx_clip_adam(float* param, float* m, float* v, float* grad, int64_t n, floa
  * with the probability that keeps their mean (rounded to nearest, a v that moves by 1 - beta2 of itself a step would never leave its code); a v > 0 below the range takes the
  * smallest code, not 0.  A block that holds an infinity, a NaN or a value of 2^127 and more reads back as NaN.  The update itself uses the moments before this rounding.
  * t: i64 [dev], the steps taken so far, counted up here (so that a captured step counts when it is replayed).
- * workspace: apx_adamw_workspace_bytes bytes, 16-byte aligned.  params / grads / m / v may have any alignment their type allows.  Sums run in a fixed order (no atomics).
- * apx_adamw_moments: 8-bit moments as the values they stand for, in bf16 (which holds them exactly). */
+ * workspace: apx_adamw_workspace_bytes bytes, 16-byte aligned.  params / grads may have any alignment
+ * their type allows, m / v and their scales are 4-byte aligned.  Sums run in a fixed order (no atomics).
+ * apx_adamw_moments: 8-bit moments as the values they stand for, in bf16 (which holds them exactly); codes 8-byte, outputs 16-byte aligned. */
 typedef struct apx_adamw_args {
     int n_tensors, grad_type, state_bits;
     float* const* params;
@@ -298,7 +299,7 @@ typedef struct apx_adamw_args {
     double* norm_out;                              /* f64 [dev] or NULL */
 } apx_adamw_args;
 int64_t apx_adamw_state_elements(int n_tensors, const int64_t* numel);
-size_t apx_adamw_workspace_bytes(int n_tensors);
+size_t apx_adamw_workspace_bytes(int n_tensors, const int64_t* numel);
 int apx_adamw(const apx_adamw_args* args, void* stream);
 int apx_adamw_moments(const void* m, const void* v, const float* m_scale, const float* v_scale, int64_t elements, void* m_out, void* v_out, void* stream);
 
