@@ -7,7 +7,9 @@
 // The channels (b, j) are independent of each other.  The backward pass needs every h_t again: the forward pass keeps the state in front of every 32nd step (f32), and the steps
 // between are run again from there.
 #include "apx_common.h"
+#include <gfx950/dynamic_lds.h>
 #include <gfx950/half_types.h>
+#include <type_traits>
 
 namespace {
 
@@ -32,9 +34,11 @@ template <> struct Elem<APX_F16> {
 
 constexpr int STEPS = 8;                  // steps of a wave in a tile: they stay in its registers
 constexpr int WAVES = 8;                  // waves of a workgroup at most
-constexpr int KEEP = 32;                  // steps between two kept states; what a tile or a segment begins with is one of them
+constexpr int KEEP = 32;                  // steps between two kept states; what a tile begins with is one of them
+constexpr int VECTOR = 2;                 // channels of a lane, where H is even
 constexpr int SEGMENTS = 256;             // parts of the time axis at most
-constexpr int FILL = 512;                 // workgroups that fill the chip: two for each CU
+constexpr int SPLIT = 128;                // steps that are worth a split at least
+constexpr int FILL = 512;                 // workgroups that fill the chip
 constexpr float LOG2E = 1.44269504088896340736f;
 
 // a = sigmoid(f) and n = 1 - a.  Whichever is below 1/2 is formed without cancellation, the other as 1 minus it, so that a + n = 1 to the last bit of the larger one: what
@@ -50,202 +54,300 @@ __device__ __forceinline__ float sigmoid(float f) { float a, n; gate(f, a, n); r
 // A run of steps is the map h -> P h + Q.  A reset inside it is P = -0: no product of gates is, products with gates keep it, and it lets nothing of h through (0 times an
 // infinity or a NaN would).
 __device__ __forceinline__ bool cut(float P) { return __float_as_uint(P) == 0x80000000u; }
-template <bool MASK> __device__ __forceinline__ float through(float P, float Q, float h) { return MASK && cut(P) ? Q : fmaf(P, h, Q); }
-
 struct alignas(8) Map { float P, Q; };
-struct Strides { int64_t t, b; };
+template <bool MASK = true> __device__ __forceinline__ float through(const Map& m, float h) { return MASK && cut(m.P) ? m.Q : fmaf(m.P, h, m.Q); }
+template <bool MASK = true> __device__ __forceinline__ Map then(const Map& m, const Map& n) {      // m first
+    return Map{MASK && cut(n.P) ? n.P : m.P * n.P, through<MASK>(n, m.Q)};
+}
+struct Strides { int64_t t, b; };         // in bytes
 struct Scan {
     int64_t T, B; int H;
     const void *f, *x, *o, *dy; void *y, *df, *dx, *do_;
     Strides sf, sx, so, sy, sdy, sdf, sdx, sdo;
     const float *h0, *dh_last; float *h_last, *save, *dh0;
     const uint8_t* reset; const int32_t* lens;
+    bool masked;                           // there are resets or lengths
     int64_t segment; int segments;         // steps of a part of the time axis (a multiple of KEEP), and how many parts
-    Map* maps;                          // [segments][B H] the parts' maps
+    Map* maps;                             // [segments][B H] the parts' maps
 };
 
 template <int TYPE, int VEC> struct Row {
     typedef typename Elem<TYPE>::raw raw;
-    struct alignas(VEC * sizeof(raw)) Pack { raw v[VEC]; };
-    static __device__ __forceinline__ Pack load(const void* base, int64_t at) { return *(const Pack*)((const raw*)base + at); }
-    static __device__ __forceinline__ float get(const Pack& p, int v) { return Elem<TYPE>::get(p.v[v]); }
-    static __device__ __forceinline__ void store(void* base, int64_t at, const float (&x)[VEC]) {
+    typedef raw Pack __attribute__((ext_vector_type(VEC), aligned(sizeof(raw))));      // (one wide access on any boundary that the type allows)
+    static __device__ __forceinline__ float get(const Pack& p, int v) { return Elem<TYPE>::get(p[v]); }
+    static __device__ __forceinline__ Pack load(const APX_GLOBAL char* wave, unsigned lane) { return *(const APX_GLOBAL Pack*)(wave + lane); }
+    static __device__ __forceinline__ void store(APX_GLOBAL char* wave, unsigned lane, const float (&x)[VEC]) {
         Pack p;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) p.v[v] = Elem<TYPE>::put(x[v]);
-        *(Pack*)((raw*)base + at) = p;
+        for (int v = 0; v < VEC; ++v) p[v] = Elem<TYPE>::put(x[v]);
+        *(APX_GLOBAL Pack*)(wave + lane) = p;
     }
 };
 
-// the VEC channels of a lane; beyond the last channel a lane reads the first ones and writes nothing
+// the VEC channels of a lane, from the first channel of its wave on; beyond the last channel a lane reads what the first lane reads and writes nothing
 template <int VEC> struct Channels {
-    int64_t c, b; int j; bool on; int64_t len;
+    int64_t c, b0, len, reach; unsigned db, j; bool on;      // reach: where the longest of the wave's sequences ends (nothing behind it is read)
     __device__ __forceinline__ Channels(const Scan& S, int group) {
-        c = ((int64_t)group * 64 + (threadIdx.x & 63)) * VEC;
+        const int64_t c0 = (int64_t)group * 64 * VEC;
+        c = c0 + (threadIdx.x & 63) * VEC;
         on = c < S.B * S.H;
-        if (!on) c = 0;
-        b = c / S.H; j = (int)(c - b * S.H);
-        len = S.lens ? (int64_t)S.lens[b] : S.T;
+        if (!on) c = c0;
+        b0 = c0 >> 32 ? c0 / S.H : (int64_t)((unsigned)c0 / (unsigned)S.H);      // (a 64-bit division is 100 instructions)
+        const unsigned in = (unsigned)(c0 - b0 * S.H) + (unsigned)(c - c0);      // channels from b0's first one on
+        db = in / (unsigned)S.H; j = in - db * (unsigned)S.H;
+        len = reach = S.T;
+        if (S.lens) {
+            const int n = S.lens[b0 + db];
+            len = n < S.T ? n : S.T;
+            int most = n;
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) { const int y = __shfl_xor(most, o, 64); most = most > y ? most : y; }
+            most = wave_uniform(most);
+            reach = most < S.T ? most : S.T;
+        }
     }
 };
+// Where an operand's rows lie: an access is a wave's address of the first of its steps (scalar registers) and 32 bits of a lane's own, one addition further with every step.  (64-bit
+// addresses in vector registers took 32 of them and two instructions an access, and one in scalar registers for each access more of those than there are.)
+struct Operand {
+    char* base; int64_t step; unsigned lane;
+    template <int VEC> __device__ __forceinline__ Operand(const void* p, const Strides& st, const Channels<VEC>& ch, unsigned bytes)
+        : base((char*)p + ch.b0 * st.b), step(st.t), lane(ch.db * (unsigned)st.b + ch.j * bytes) {}
+    __device__ __forceinline__ APX_GLOBAL char* at(int64_t t) const { return wave_address(base + t * step); }
+    __device__ __forceinline__ unsigned offset(int i) const { return lane_offset(lane + (unsigned)i * (unsigned)step); }
+};
 
-// a, n of one step of a lane's channels as the maps need them: keep = -0 at a reset, 1 and n = 0 where the step does not count
-template <bool MASK> __device__ __forceinline__ void step_gate(float f, bool counts, bool reset, float& a, float& keep, float& n) {
-    gate(f, a, n);
-    keep = MASK && reset ? -0.f : a;
-    if (!counts) { keep = a = 1.f; n = 0.f; }
+// What a step counts for: everything, or - behind a sequence's end, behind the part's - nothing: then a = 1 and n = 0.  Nearly every tile of a wave counts in whole and holds no
+// reset; one vote of the wave decides between that form of the arithmetic and the one with the masks (twice the instructions).
+typedef std::integral_constant<bool, false> Plain;
+typedef std::integral_constant<bool, true> Masked;
+__device__ __forceinline__ bool nowhere(bool x) { return __builtin_amdgcn_ballot_w64(x) == 0; }
+
+// how many of the STEPS steps from t0 on lie in front of `end`
+__device__ __forceinline__ int steps_left(int64_t t0, int64_t end) { return t0 >= end ? 0 : end - t0 < STEPS ? (int)(end - t0) : STEPS; }
+// those steps of a lane (at least one; the last one again beyond them)
+template <class R> __device__ __forceinline__ void load_steps(typename R::Pack (&q)[STEPS], const Operand& o, int64_t t0, int left) {
+    const APX_GLOBAL char* p = o.at(t0);
+    unsigned at = o.offset(0);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        q[i] = R::load(p, at);
+        at += i + 1 < left ? (unsigned)o.step : 0u;
+    }
+}
+__device__ __forceinline__ void load_resets(uint8_t (&r)[STEPS], const Scan& S, const Operand& o, int64_t t0, int left) {
+    if (!S.reset) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) r[i] = 0;
+        return;
+    }
+    const APX_GLOBAL char* p = o.at(t0);
+    unsigned at = o.offset(0);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        r[i] = (uint8_t)p[at];
+        at += i + 1 < left ? (unsigned)o.step : 0u;
+    }
+}
+// the steps that are resets, as bits
+__device__ __forceinline__ unsigned reset_bits(const uint8_t (&r)[STEPS]) {
+    unsigned bits = 0;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) bits |= (r[i] ? 1u : 0u) << i;
+    return bits;
+}
+// how many of a lane's steps count, and whether in the whole wave all do and none is a reset
+template <int VEC> __device__ __forceinline__ bool plain_steps(const Scan& S, const Channels<VEC>& ch, unsigned resets, int64_t t0, int left, int& live) {
+    live = left;
+    if (S.masked) live = t0 >= ch.len ? 0 : ch.len - t0 < left ? (int)(ch.len - t0) : left;
+    return left == STEPS && (!S.masked || nowhere(resets != 0 || live < STEPS));
 }
 
-// ------------------------------------------------------------------------------------------------ the maps of the parts (only where the time axis is split)
-// forward: h behind the part from h in front of it; BACK: c in front of it from c behind it.  A wave takes a contiguous share of the part.
-template <int TYPE, int VEC, bool GATE, bool MASK, bool BACK>
+// maps of the waves of a workgroup, two tiles' worth in turn: [2][waves][64 VEC] Map forward, [2][waves][3][64 VEC] floats backward (sized by the launch: a static array for WAVES
+// waves would keep workgroups of fewer waves off the CU)
+APX_DYNAMIC_LDS(Map, scan_lds, 16);
+
+// ------------------------------------------------------------------------------------------------ a split time axis
+// The maps of the parts.  Forward: h behind the part from h in front of it; BACK: c in front of it from c behind it.  A wave takes a contiguous share of the part, STEPS steps at a
+// time, the next ones on their way meanwhile.
+template <int TYPE, int VEC, bool GATE, bool BACK>
 __global__ __launch_bounds__(64 * WAVES) void gated_scan_maps_kernel(Scan S) {
     typedef Row<TYPE, VEC> R;
-    __shared__ Map L[WAVES][64 * VEC];
+    Map* L = scan_lds;
     const int lane = threadIdx.x & 63, w = wave_uniform(threadIdx.x >> 6), nw = blockDim.x >> 6;
     const Channels<VEC> ch(S, blockIdx.x);
     const int64_t begin = (int64_t)blockIdx.y * S.segment, end = begin + S.segment < S.T ? begin + S.segment : S.T;
     const int64_t share = (S.segment / nw + STEPS - 1) / STEPS * STEPS;
-    const int64_t t0 = begin + w * share, t1 = t0 + share < end ? t0 + share : end;
-    float P[VEC], Q[VEC];
+    const int64_t stop = end < ch.reach ? end : ch.reach, first = begin + w * share, last = first + share < stop ? first + share : stop;
+    const unsigned e = sizeof(typename R::raw);
+    const Operand of(S.f, S.sf, ch, e), oq(BACK ? S.dy : S.x, BACK ? S.sdy : S.sx, ch, e), oo(S.o, S.so, ch, e), orst(S.reset, Strides{S.B, 1}, ch, 0);
+    Map m[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) { P[v] = 1.f; Q[v] = 0.f; }
-    for (int64_t k = 0; k < share && t0 < end; k += STEPS) {
+    for (int v = 0; v < VEC; ++v) m[v] = Map{1.f, 0.f};
+    if (first < last) {
         typename R::Pack f[STEPS], q[STEPS], o[GATE ? STEPS : 1];
-        bool rs[STEPS];
+        uint8_t rs[STEPS];
+        auto fetch = [&](int64_t t0) {
+            const int left = steps_left(t0, last);
+            load_steps<R>(f, of, t0, left);
+            load_steps<R>(q, oq, t0, left);
+            if constexpr (GATE) load_steps<R>(o, oo, t0, left);
+            load_resets(rs, S, orst, t0, left);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        const int64_t tiles = (last - first + STEPS - 1) / STEPS;
+        fetch(first + (BACK ? tiles - 1 : 0) * STEPS);
+        for (int64_t k = 0; k < tiles; ++k) {
+            const int64_t t0 = first + (BACK ? tiles - 1 - k : k) * STEPS;
+            const unsigned resets = reset_bits(rs);
+            int live;
+            const bool plain = plain_steps(S, ch, resets, t0, steps_left(t0, last), live);
+            Map one[STEPS][VEC];
+            auto steps = [&](auto masked) {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const int64_t u = BACK ? t1 - 1 - k - i : t0 + k + i;
-            const int64_t t = u < t0 ? t0 : u < t1 ? u : t1 - 1;
-            f[i] = R::load(S.f, t * S.sf.t + ch.b * S.sf.b + ch.j);
-            q[i] = BACK ? R::load(S.dy, t * S.sdy.t + ch.b * S.sdy.b + ch.j) : R::load(S.x, t * S.sx.t + ch.b * S.sx.b + ch.j);
-            if (GATE) o[i] = R::load(S.o, t * S.so.t + ch.b * S.so.b + ch.j);
-            rs[i] = MASK && S.reset && S.reset[t * S.B + ch.b];
-        }
+                for (int i = 0; i < STEPS; ++i) {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const int64_t u = BACK ? t1 - 1 - k - i : t0 + k + i;
-            const bool counts = u >= t0 && u < t1 && (!MASK || u < ch.len);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float a, keep, n;
-                step_gate<MASK>(R::get(f[i], v), counts, rs[i], a, keep, n);
-                if (BACK) {      // c -> keep (d + c)
-                    const float d = GATE ? R::get(q[i], v) * sigmoid(R::get(o[i], v)) : R::get(q[i], v);
-                    const float s = counts ? d + Q[v] : Q[v];
-                    Q[v] = MASK && cut(keep) ? 0.f : keep * s;
-                } else {
-                    const float b = counts ? n * R::get(q[i], v) : 0.f;
-                    Q[v] = through<MASK>(keep, b, Q[v]);
+                    for (int v = 0; v < VEC; ++v) {
+                        float a, n;
+                        gate(R::get(f[i], v), a, n);
+                        float x = R::get(q[i], v);
+                        if constexpr (GATE) x *= sigmoid(R::get(o[i], v));
+                        one[i][v] = Map{a, BACK ? a * x : n * x};      // BACK: c -> a (d + c)
+                        if (masked) {
+                            if (resets >> i & 1u) one[i][v] = Map{-0.f, BACK ? 0.f : one[i][v].Q};
+                            if (i >= live) one[i][v] = Map{1.f, 0.f};
+                        }
+                    }
                 }
-                P[v] = MASK && cut(keep) ? keep : P[v] * keep;
-            }
+            };
+            if (plain) steps(Plain()); else steps(Masked());
+            if (k + 1 < tiles) fetch(first + (BACK ? tiles - 2 - k : k + 1) * STEPS);
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) m[v] = plain ? then<false>(m[v], one[BACK ? STEPS - 1 - i : i][v]) : then(m[v], one[BACK ? STEPS - 1 - i : i][v]);
         }
     }
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) L[w][lane * VEC + v] = Map{P[v], Q[v]};
+    for (int v = 0; v < VEC; ++v) L[(w * 64 + lane) * VEC + v] = m[v];
     __syncthreads();
     if (w == 0 && ch.on) {
         Map* out = S.maps + (int64_t)blockIdx.y * S.B * S.H + ch.c;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            float p = 1.f, q = 0.f;
-            for (int i = 0; i < nw; ++i) {
-                const Map m = L[BACK ? nw - 1 - i : i][lane * VEC + v];
-                q = through<MASK>(m.P, m.Q, q);
-                p = MASK && cut(m.P) ? m.P : p * m.P;
-            }
-            out[v] = Map{p, q};
+            Map all = {1.f, 0.f};
+            for (int i = 0; i < nw; ++i) all = then(all, L[((BACK ? nw - 1 - i : i) * 64 + lane) * VEC + v]);
+            out[v] = all;
         }
     }
 }
 
 // what enters a part: `h` carried through the maps of the parts [0, part) - or, BACK, (part, segments) from the last -, a contiguous share of them in each wave
-template <int VEC, bool MASK, bool BACK>
+template <int VEC, bool BACK>
 __device__ __forceinline__ void enter(const Scan& S, const Channels<VEC>& ch, int part, int w, int nw, Map* L, float (&h)[VEC]) {
     const int lane = threadIdx.x & 63, count = BACK ? S.segments - 1 - part : part;
     if (count == 0) return;
     const int share = (count + nw - 1) / nw, i0 = w * share, i1 = i0 + share < count ? i0 + share : count;
-    float P[VEC], Q[VEC];
+    Map m[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) { P[v] = 1.f; Q[v] = 0.f; }
-    for (int i = i0; i < i1; ++i) {
-        const Map* m = S.maps + (int64_t)(BACK ? S.segments - 1 - i : i) * S.B * S.H + ch.c;
+    for (int v = 0; v < VEC; ++v) m[v] = Map{1.f, 0.f};
+    for (int i = i0; i < i1; i += 4) {
+        Map q[4][VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const Map q = m[v];
-            Q[v] = through<MASK>(q.P, q.Q, Q[v]);
-            P[v] = MASK && cut(q.P) ? q.P : P[v] * q.P;
+        for (int k = 0; k < 4; ++k) {
+            const int at = i + k < i1 ? i + k : i;
+            const Map* p = S.maps + (int64_t)(BACK ? S.segments - 1 - at : at) * S.B * S.H + ch.c;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) q[k][v] = p[v];
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) if (i + k < i1) m[v] = then(m[v], q[k][v]);
     }
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) L[w * 64 * VEC + lane * VEC + v] = Map{P[v], Q[v]};
+    for (int v = 0; v < VEC; ++v) L[w * 64 * VEC + lane * VEC + v] = m[v];
     __syncthreads();
     for (int i = 0; i < nw; ++i)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const Map m = L[i * 64 * VEC + lane * VEC + v];
-            h[v] = through<MASK>(m.P, m.Q, h[v]);
-        }
+        for (int v = 0; v < VEC; ++v) h[v] = through(L[i * 64 * VEC + lane * VEC + v], h[v]);
     __syncthreads();
 }
 
 // ------------------------------------------------------------------------------------------------ forward
 // A workgroup walks a part of the time axis of 64 VEC channels in tiles of nw x STEPS steps.  A wave holds its STEPS steps of a tile in registers, the maps of the waves' steps
 // meet in LDS (one barrier a tile, two buffers in turn), each wave then runs its own steps again from the state that enters them: one read of the inputs, no step of the chain
-// longer than STEPS + nw multiply-adds.
-template <int TYPE, int VEC, bool GATE, bool MASK>
+// longer than STEPS + nw multiply-adds.  Without an output gate the next tile's loads are issued before this one's barrier (with one there are not the registers for it).
+template <int TYPE, int VEC, bool GATE>
 __global__ __launch_bounds__(64 * WAVES) void gated_scan_fwd_kernel(Scan S) {
     typedef Row<TYPE, VEC> R;
-    __shared__ Map L[2][WAVES][64 * VEC];
+    constexpr bool AHEAD = !GATE;
+    Map* L = scan_lds;
     const int lane = threadIdx.x & 63, w = wave_uniform(threadIdx.x >> 6), nw = blockDim.x >> 6;
     const Channels<VEC> ch(S, blockIdx.x);
-    const int64_t begin = (int64_t)blockIdx.y * S.segment, end = begin + S.segment < S.T ? begin + S.segment : S.T;
+    const int64_t step = nw * STEPS, begin = (int64_t)blockIdx.y * S.segment, end = begin + S.segment < S.T ? begin + S.segment : S.T;
     float h[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) h[v] = S.h0 ? S.h0[ch.c + v] : 0.f;
-    enter<VEC, MASK, false>(S, ch, blockIdx.y, w, nw, &L[0][0][0], h);
+    const unsigned e = sizeof(typename R::raw);
+    const Operand of(S.f, S.sf, ch, e), ox(S.x, S.sx, ch, e), oo(S.o, S.so, ch, e), oy(S.y, S.sy, ch, e), orst(S.reset, Strides{S.B, 1}, ch, 0);
+    typename R::Pack f[STEPS], x[STEPS], o[GATE ? STEPS : 1];
+    uint8_t rs[STEPS];
+    const int64_t stop = end < ch.reach ? end : ch.reach;
+    auto fetch = [&](int64_t t0) {
+        const int left = steps_left(t0, stop);
+        if (left == 0) return;
+        load_steps<R>(f, of, t0, left);
+        load_steps<R>(x, ox, t0, left);
+        if constexpr (GATE) load_steps<R>(o, oo, t0, left);
+        load_resets(rs, S, orst, t0, left);
+        __builtin_amdgcn_sched_barrier(0);
+    };
     int turn = 0;
-    for (int64_t tile = begin; tile < end; tile += nw * STEPS, turn ^= 1) {
+    if (AHEAD && begin < end) fetch(begin + w * STEPS);
+    enter<VEC, false>(S, ch, blockIdx.y, w, nw, L, h);
+    for (int64_t tile = begin; tile < end; tile += step, turn ^= 1) {
         const int64_t t0 = tile + w * STEPS;
-        float a[STEPS][VEC], b[STEPS][VEC], s[GATE ? STEPS : 1][VEC], P[VEC], Q[VEC];
-        {
-            typename R::Pack f[STEPS], x[STEPS], o[GATE ? STEPS : 1];
-            bool rs[STEPS];
+        if (!AHEAD) fetch(t0);
+        Map one[STEPS][VEC], m[VEC];
+        const unsigned resets = reset_bits(rs);
+        const int left = steps_left(t0, end);
+        int live;
+        const bool plain = plain_steps(S, ch, resets, t0, left, live);
+        const bool none = t0 >= stop;
+        if (none) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) m[v] = Map{1.f, 0.f};
+        }
+        auto maps = [&](auto masked) {
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) {
-                const int64_t t = t0 + i < end ? t0 + i : end - 1;
-                f[i] = R::load(S.f, t * S.sf.t + ch.b * S.sf.b + ch.j);
-                x[i] = R::load(S.x, t * S.sx.t + ch.b * S.sx.b + ch.j);
-                if (GATE) o[i] = R::load(S.o, t * S.so.t + ch.b * S.so.b + ch.j);
-                rs[i] = MASK && S.reset && S.reset[t * S.B + ch.b];
-            }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) { P[v] = 1.f; Q[v] = 0.f; }
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                const bool counts = t0 + i < end && (!MASK || t0 + i < ch.len);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    float g, n;
-                    step_gate<MASK>(R::get(f[i], v), counts, rs[i], g, a[i][v], n);
-                    b[i][v] = counts ? n * R::get(x[i], v) : 0.f;
-                    Q[v] = through<MASK>(a[i][v], b[i][v], Q[v]);
-                    P[v] = MASK && cut(a[i][v]) ? a[i][v] : P[v] * a[i][v];
-                    if (GATE) s[i][v] = sigmoid(R::get(o[i], v));
+                    float a, n;
+                    gate(R::get(f[i], v), a, n);
+                    one[i][v] = Map{a, n * R::get(x[i], v)};
+                    if (masked) {
+                        if (resets >> i & 1u) one[i][v].P = -0.f;
+                        if (i >= live) one[i][v] = Map{1.f, 0.f};
+                    }
+                    m[v] = i == 0 ? one[i][v] : then<masked>(m[v], one[i][v]);
                 }
             }
-        }
+        };
+        if (plain) maps(Plain()); else if (!none) maps(Masked());
+        if (AHEAD && tile + step < end) fetch(t0 + step);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) L[turn][w][lane * VEC + v] = Map{P[v], Q[v]};
+        for (int v = 0; v < VEC; ++v) L[((turn * nw + w) * 64 + lane) * VEC + v] = m[v];
         __syncthreads();
         float in[VEC];
+#pragma unroll 4
         for (int i = 0; i < nw; ++i) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 if (i == w) in[v] = h[v];
-                const Map m = L[turn][i][lane * VEC + v];
-                h[v] = through<MASK>(m.P, m.Q, h[v]);
+                const Map k = L[((turn * nw + i) * 64 + lane) * VEC + v];
+                h[v] = S.masked ? through(k, h[v]) : through<false>(k, h[v]);
             }
         }
         if (!ch.on) continue;
@@ -253,20 +355,31 @@ __global__ __launch_bounds__(64 * WAVES) void gated_scan_fwd_kernel(Scan S) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) S.save[(t0 / KEEP) * S.B * S.H + ch.c + v] = in[v];
         }
+        APX_GLOBAL char* const py = oy.at(t0);
+        unsigned at = oy.offset(0);
+        auto outputs = [&](auto masked) {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            if (t0 + i >= end) break;
-            float y[VEC];
+            for (int i = 0; i < STEPS; ++i, at += (unsigned)oy.step) {
+                if (masked && i >= left) break;
+                float y[VEC];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                in[v] = through<MASK>(a[i][v], b[i][v], in[v]);
-                y[v] = GATE ? in[v] * s[i][v] : in[v];
-                if (MASK && t0 + i >= ch.len) y[v] = 0.f;
+                for (int v = 0; v < VEC; ++v) {
+                    in[v] = through<masked>(one[i][v], in[v]);
+                    y[v] = in[v];
+                    if constexpr (GATE) y[v] *= sigmoid(R::get(o[i], v));
+                    if (masked && i >= live) y[v] = 0.f;
+                }
+                R::store(py, at, y);
             }
-            R::store(S.y, (t0 + i) * S.sy.t + ch.b * S.sy.b + ch.j, y);
+        };
+        if (plain) outputs(Plain());
+        else if (!none) outputs(Masked());
+        else {
+            const float zero[VEC] = {};
+            for (int i = 0; i < left; ++i, at += (unsigned)oy.step) R::store(py, at, zero);
         }
     }
-    if (w == 0 && ch.on && blockIdx.y == S.segments - 1) {
+    if (w == 0 && ch.on && end == S.T) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) S.h_last[ch.c + v] = h[v];
     }
@@ -275,115 +388,152 @@ __global__ __launch_bounds__(64 * WAVES) void gated_scan_fwd_kernel(Scan S) {
 // ------------------------------------------------------------------------------------------------ backward
 // The same walk from the end.  A tile begins with a kept state; the waves' maps of h (forward in time) and of c (backward: the same product of gates) meet in LDS together.  A wave
 // then runs its steps forward for the states and backward for the gradients, on registers alone.
-template <int TYPE, int VEC, bool GATE, bool MASK>
+template <int TYPE, int VEC, bool GATE>
 __global__ __launch_bounds__(64 * WAVES) void gated_scan_bwd_kernel(Scan S) {
     typedef Row<TYPE, VEC> R;
-    __shared__ float L[2][WAVES][3][64 * VEC];
+    constexpr bool AHEAD = !GATE;
+    float* const L = (float*)(Map*)scan_lds;
     const int lane = threadIdx.x & 63, w = wave_uniform(threadIdx.x >> 6), nw = blockDim.x >> 6;
     const Channels<VEC> ch(S, blockIdx.x);
-    const int64_t begin = (int64_t)blockIdx.y * S.segment, end = begin + S.segment < S.T ? begin + S.segment : S.T;
+    const int64_t step = nw * STEPS, begin = (int64_t)blockIdx.y * S.segment, end = begin + S.segment < S.T ? begin + S.segment : S.T;
     float c[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) c[v] = S.dh_last ? S.dh_last[ch.c + v] : 0.f;
-    enter<VEC, MASK, true>(S, ch, blockIdx.y, w, nw, (Map*)&L[0][0][0][0], c);
-    int turn = 0;
-    const int64_t step = nw * STEPS;
-    for (int64_t tile = begin + (end - begin - 1) / step * step; tile >= begin && end > begin; tile -= step, turn ^= 1) {
+    const unsigned e = sizeof(typename R::raw);
+    const Operand of(S.f, S.sf, ch, e), ox(S.x, S.sx, ch, e), ody(S.dy, S.sdy, ch, e), oo(S.o, S.so, ch, e), odf(S.df, S.sdf, ch, e), odx(S.dx, S.sdx, ch, e), odo(S.do_, S.sdo, ch, e),
+        orst(S.reset, Strides{S.B, 1}, ch, 0);
+    typename R::Pack rf[STEPS], rx[STEPS], rd[STEPS], ro[GATE ? STEPS : 1];
+    uint8_t rs[STEPS];
+    float kept[VEC];
+    const int64_t stop = end < ch.reach ? end : ch.reach;
+    auto fetch = [&](int64_t tile) {
         const int64_t t0 = tile + w * STEPS;
-        // of each step: the gate and 1 minus it, x - later (p - x) a n -, the gradient d of the state's own output; of the output gate the smaller of
-        // it and 1 minus it (their product is its derivative, formed without cancellation)
-        float a[STEPS][VEC], n[STEPS][VEC], x[STEPS][VEC], d[STEPS][VEC], s[GATE ? STEPS : 1][VEC], dy[GATE ? STEPS : 1][VEC], h[VEC];
-        unsigned resets = 0;
-        {
-            typename R::Pack rf[STEPS], rx[STEPS], rd[STEPS], ro[GATE ? STEPS : 1];
+        const int left = steps_left(t0, stop);
+        if (left == 0) return;
+        load_steps<R>(rf, of, t0, left);
+        load_steps<R>(rx, ox, t0, left);
+        load_steps<R>(rd, ody, t0, left);
+        if constexpr (GATE) load_steps<R>(ro, oo, t0, left);
+        load_resets(rs, S, orst, t0, left);
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                const int64_t t = t0 + i < end ? t0 + i : end - 1;
-                rf[i] = R::load(S.f, t * S.sf.t + ch.b * S.sf.b + ch.j);
-                rx[i] = R::load(S.x, t * S.sx.t + ch.b * S.sx.b + ch.j);
-                rd[i] = R::load(S.dy, t * S.sdy.t + ch.b * S.sdy.b + ch.j);
-                if (GATE) ro[i] = R::load(S.o, t * S.so.t + ch.b * S.so.b + ch.j);
-                if (MASK && S.reset) resets |= (S.reset[t * S.B + ch.b] && t0 + i < end && t0 + i < ch.len ? 1u : 0u) << i;
-            }
+        for (int v = 0; v < VEC; ++v) kept[v] = S.save[(tile / KEEP) * S.B * S.H + ch.c + v];
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    int turn = 0;
+    auto at = [&](int wave, int k) { return L + (((turn * nw + wave) * 3 + k) * 64 + lane) * VEC; };
+    const int64_t last = begin + (end - begin - 1) / step * step;
+    if (AHEAD && begin < end) fetch(last);
+    enter<VEC, true>(S, ch, blockIdx.y, w, nw, scan_lds, c);
+    for (int64_t tile = last; tile >= begin && end > begin; tile -= step, turn ^= 1) {
+        const int64_t t0 = tile + w * STEPS;
+        if (!AHEAD) fetch(tile);
+        // of each step: the gate and 1 minus it, x - later (p - x) a n -, and dy - later the gradient of the state's own output, dy sigmoid(o)
+        float a[STEPS][VEC], n[STEPS][VEC], x[STEPS][VEC], d[STEPS][VEC], h[VEC];
+        const unsigned resets = reset_bits(rs);
+        const int left = steps_left(t0, end);
+        int live;
+        const bool plain = plain_steps(S, ch, resets, t0, left, live);
+        const bool none = t0 >= stop;
+        if (none) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = S.save[(tile / KEEP) * S.B * S.H + ch.c + v];
+            for (int v = 0; v < VEC; ++v) { at(w, 0)[v] = 1.f; at(w, 1)[v] = at(w, 2)[v] = h[v] = 0.f; }
+        }
+        auto maps = [&](auto masked) {
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                const bool counts = t0 + i < end && (!MASK || t0 + i < ch.len);
+            for (int v = 0; v < VEC; ++v) {
+                float P = 1.f, Q = 0.f, C = 0.f;
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) {
+                for (int i = 0; i < STEPS; ++i) {
+                    const bool counts = !masked || i < live, reset = masked && counts && (resets >> i & 1u);
                     gate(R::get(rf[i], v), a[i][v], n[i][v]);
                     if (!counts) { a[i][v] = 1.f; n[i][v] = 0.f; }
                     x[i][v] = counts ? R::get(rx[i], v) : 0.f;
                     const float y = counts ? R::get(rd[i], v) : 0.f;
-                    if (GATE) {
-                        float g, r;
-                        gate(R::get(ro[i], v), g, r);
-                        s[i][v] = g < r ? g : r;
-                        dy[i][v] = y; d[i][v] = counts ? y * g : 0.f;
-                    } else d[i][v] = y;
+                    d[i][v] = y;
+                    const float b = n[i][v] * x[i][v];
+                    Q = reset ? b : fmaf(a[i][v], Q, b);
+                    P = reset ? -0.f : P * a[i][v];
                 }
+#pragma unroll
+                for (int i = STEPS - 1; i >= 0; --i) {
+                    float g = d[i][v];
+                    if constexpr (GATE) { g *= sigmoid(R::get(ro[i], v)); if (masked && i >= live) g = 0.f; }
+                    C = masked && (resets >> i & 1u) && i < live ? 0.f : a[i][v] * (g + C);
+                }
+                at(w, 0)[v] = P; at(w, 1)[v] = Q; at(w, 2)[v] = C;
+                h[v] = kept[v];
             }
-        }
-        auto reset = [&](int i) { return MASK && (resets >> i & 1u); };
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            float P = 1.f, Q = 0.f, B = 0.f;
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                const float b = n[i][v] * x[i][v];
-                Q = reset(i) ? b : fmaf(a[i][v], Q, b);
-                P = reset(i) ? -0.f : P * a[i][v];
-            }
-#pragma unroll
-            for (int i = STEPS - 1; i >= 0; --i) B = reset(i) ? 0.f : a[i][v] * (d[i][v] + B);
-            L[turn][w][0][lane * VEC + v] = P; L[turn][w][1][lane * VEC + v] = Q; L[turn][w][2][lane * VEC + v] = B;
-        }
+        };
+        if (plain) maps(Plain()); else if (!none) maps(Masked());
+        if (AHEAD && tile > begin) fetch(tile - step);
         __syncthreads();
         float cin[VEC];
+        auto fold = [&](auto masked) {
+#pragma unroll 2
+            for (int i = 0; i < w; ++i)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            for (int i = 0; i < w; ++i) h[v] = through<MASK>(L[turn][i][0][lane * VEC + v], L[turn][i][1][lane * VEC + v], h[v]);
-            for (int i = nw - 1; i >= 0; --i) {
-                if (i == w) cin[v] = c[v];
-                c[v] = through<MASK>(L[turn][i][0][lane * VEC + v], L[turn][i][2][lane * VEC + v], c[v]);
-            }
-        }
-        if (!ch.on) continue;
+                for (int v = 0; v < VEC; ++v) h[v] = through<masked>(Map{at(i, 0)[v], at(i, 1)[v]}, h[v]);
+#pragma unroll 2
+            for (int i = nw - 1; i >= 0; --i)
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            if (t0 + i >= end) break;
-            float out[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float p = reset(i) ? 0.f : h[v];
-                h[v] = fmaf(a[i][v], p, n[i][v] * x[i][v]);
-                x[i][v] = (p - x[i][v]) * a[i][v] * n[i][v];
-                if (GATE) {
-                    const float r = s[i][v];
-                    out[v] = dy[i][v] * h[v] * r * (1.f - r);
-                    if (MASK && t0 + i >= ch.len) out[v] = 0.f;
+                for (int v = 0; v < VEC; ++v) {
+                    if (i == w) cin[v] = c[v];
+                    c[v] = through<masked>(Map{at(i, 0)[v], at(i, 2)[v]}, c[v]);
                 }
-            }
-            if (GATE) R::store(S.do_, (t0 + i) * S.sdo.t + ch.b * S.sdo.b + ch.j, out);
-        }
+        };
+        if (S.masked) fold(Masked()); else fold(Plain());
+        if (!ch.on) continue;
+        APX_GLOBAL char *const pdo = odo.at(t0), *const pdf = odf.at(t0), *const pdx = odx.at(t0);
+        unsigned ado = odo.offset(0), adf = odf.offset(STEPS - 1), adx = odx.offset(STEPS - 1);
+        auto outputs = [&](auto masked) {
+            auto counts = [&](int i) { return !masked || i < live; };
+            auto reset = [&](int i) { return masked && (resets >> i & 1u) && counts(i); };
 #pragma unroll
-        for (int i = STEPS - 1; i >= 0; --i) {
-            float df[VEC], dx[VEC];
+            for (int i = 0; i < STEPS; ++i) {
+                float out[VEC];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float g = d[i][v] + cin[v];
-                dx[v] = n[i][v] * g; df[v] = x[i][v] * g;
-                if (MASK && t0 + i >= ch.len) dx[v] = df[v] = 0.f;
-                cin[v] = reset(i) ? 0.f : a[i][v] * g;
+                for (int v = 0; v < VEC; ++v) {
+                    const float p = reset(i) ? 0.f : h[v];
+                    h[v] = fmaf(a[i][v], p, n[i][v] * x[i][v]);
+                    x[i][v] = (p - x[i][v]) * (a[i][v] * n[i][v]);
+                    if constexpr (GATE) {
+                        float g, r;
+                        gate(R::get(ro[i], v), g, r);
+                        out[v] = counts(i) ? d[i][v] * h[v] * (g * r) : 0.f;
+                        d[i][v] = counts(i) ? d[i][v] * g : 0.f;
+                    }
+                }
+                if constexpr (GATE) { if (!masked || i < left) R::store(pdo, ado, out); ado += (unsigned)odo.step; }
             }
-            if (t0 + i < end) {
-                R::store(S.df, (t0 + i) * S.sdf.t + ch.b * S.sdf.b + ch.j, df);
-                R::store(S.dx, (t0 + i) * S.sdx.t + ch.b * S.sdx.b + ch.j, dx);
+#pragma unroll
+            for (int i = STEPS - 1; i >= 0; --i) {
+                float df[VEC], dx[VEC];
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    const float g = d[i][v] + cin[v];
+                    dx[v] = n[i][v] * g; df[v] = x[i][v] * g;
+                    if (!counts(i)) dx[v] = df[v] = 0.f;
+                    cin[v] = reset(i) ? 0.f : a[i][v] * g;
+                }
+                if (!masked || i < left) {
+                    R::store(pdf, adf, df);
+                    R::store(pdx, adx, dx);
+                }
+                adf -= (unsigned)odf.step; adx -= (unsigned)odx.step;
+            }
+        };
+        if (plain) outputs(Plain());
+        else if (!none) outputs(Masked());
+        else {
+            const float zero[VEC] = {};
+            for (int i = 0; i < left; ++i) {
+                R::store(pdf, odf.offset(i), zero);
+                R::store(pdx, odx.offset(i), zero);
+                if constexpr (GATE) R::store(pdo, odo.offset(i), zero);
             }
         }
     }
-    if (w == 0 && ch.on && blockIdx.y == 0 && S.dh0) {
+    if (w == 0 && ch.on && begin == 0 && S.dh0) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) S.dh0[ch.c + v] = c[v];
     }
@@ -396,12 +546,13 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(Scan S, float* __r
     const int64_t c = blockIdx.x * (int64_t)256 + threadIdx.x;
     if (c >= S.B * S.H) return;
     const int64_t b = c / S.H; const int j = (int)(c - b * S.H);
+    auto at = [&](const void* p, const Strides& st) { return *(const raw*)((const char*)p + b * st.b + j * sizeof(raw)); };
     float a, n;
-    gate(E::get(((const raw*)S.f)[b * S.sf.b + j]), a, n);
-    const float v = n * E::get(((const raw*)S.x)[b * S.sx.b + j]);
+    gate(E::get(at(S.f, S.sf)), a, n);
+    const float v = n * E::get(at(S.x, S.sx));
     const float s = S.reset && S.reset[b] ? v : fmaf(a, h[c], v);
     h[c] = s;
-    ((raw*)S.y)[b * S.sy.b + j] = E::put(S.o ? s * sigmoid(E::get(((const raw*)S.o)[b * S.so.b + j])) : s);
+    *(raw*)((char*)S.y + b * S.sy.b + j * sizeof(raw)) = E::put(S.o ? s * sigmoid(E::get(at(S.o, S.so))) : s);
 }
 
 // entries (t, b, j) of an output do not fall on each other: either whole steps follow one another or whole sequences do
@@ -421,13 +572,13 @@ bool reaches(int64_t T, int64_t B, int H, int64_t st, int64_t sb) {
 #define APX_SCAN_WORKSPACE()                                                                                              \
     do {                                                                                                                  \
         const size_t need = apx_gated_scan_workspace_bytes(a->T, a->B, a->H);                                             \
-        APX_REQUIRE(need == 0 || (a->workspace && ((uintptr_t)a->workspace & 15) == 0 && a->workspace_bytes >= need), "workspace"); \
+        APX_REQUIRE(need == 0 || (a->workspace && ((uintptr_t)a->workspace & 15) == 0 && a->workspace_bytes >= need), "workspace");                \
     } while (0)
 
 int check_common(const apx_gated_scan_args* a) {
     APX_REQUIRE(a, "args");
     APX_REQUIRE(a->type == APX_F32 || a->type == APX_BF16 || a->type == APX_F16, "type");
-    APX_REQUIRE(a->T >= 0 && a->B >= 0 && a->H >= 0, "T, B, H");
+    APX_REQUIRE(a->T >= 0 && a->B >= 0 && a->H >= 0 && a->T < ((int64_t)1 << 40), "T, B, H");
     APX_REQUIRE((__int128)a->B * a->H < ((__int128)1 << 36), "B * H");
     APX_REQUIRE((__int128)a->B * a->H * (a->T + 1) < ((__int128)1 << 59), "T * B * H");
     return APX_OK;
@@ -436,65 +587,62 @@ Scan scan_of(const apx_gated_scan_args* a) {
     Scan S = {};
     S.T = a->T; S.B = a->B; S.H = a->H;
     S.f = a->f; S.x = a->x; S.o = a->o; S.dy = a->dy; S.y = a->y; S.df = a->df; S.dx = a->dx; S.do_ = a->do_;
-    S.sf = {a->f_t, a->f_b}; S.sx = {a->x_t, a->x_b}; S.so = {a->o_t, a->o_b}; S.sy = {a->y_t, a->y_b};
-    S.sdy = {a->dy_t, a->dy_b}; S.sdf = {a->df_t, a->df_b}; S.sdx = {a->dx_t, a->dx_b}; S.sdo = {a->do_t, a->do_b};
+    const int64_t e = a->type == APX_F32 ? 4 : 2;
+    S.sf = {a->f_t * e, a->f_b * e}; S.sx = {a->x_t * e, a->x_b * e}; S.so = {a->o_t * e, a->o_b * e}; S.sy = {a->y_t * e, a->y_b * e};
+    S.sdy = {a->dy_t * e, a->dy_b * e}; S.sdf = {a->df_t * e, a->df_b * e}; S.sdx = {a->dx_t * e, a->dx_b * e}; S.sdo = {a->do_t * e, a->do_b * e};
     S.h0 = a->h0; S.dh_last = a->dh_last; S.h_last = a->h_last; S.save = a->save; S.dh0 = a->dh0;
     S.reset = a->reset; S.lens = a->lens;
     return S;
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-// How the time axis is split: where the channels alone do not fill the chip, into parts of at least two tiles' steps (a part costs a second look at f and x, and each part folds the
-// maps of the parts before it).
+// How the time axis is split: where the channels alone do not fill the chip, into parts of whole kept stretches (a part costs a second look at f and x, and folds the maps of the
+// parts before it).
 struct Split { int64_t groups, segment; int segments; };
 Split split(int64_t T, int64_t BH, int vec) {
     Split p;
     p.groups = (BH + 64 * vec - 1) / (64 * vec);
-    int64_t want = p.groups >= FILL / 2 ? 1 : FILL / p.groups;
-    const int64_t most = T / (WAVES * STEPS);
-    if (want > most) want = most;
+    int64_t want = T < SPLIT || p.groups >= FILL / 2 ? 1 : FILL / p.groups;
+    if (want > T / KEEP) want = T / KEEP;
     if (want > SEGMENTS) want = SEGMENTS;
-    if (want < 2) { p.segment = (T + KEEP - 1) / KEEP * KEEP; if (p.segment == 0) p.segment = KEEP; p.segments = 1; return p; }
+    if (want < 2) want = 1;
     p.segment = ((T + want - 1) / want + KEEP - 1) / KEEP * KEEP;
-    p.segments = (int)((T + p.segment - 1) / p.segment);
+    if (p.segment == 0) p.segment = KEEP;
+    p.segments = T ? (int)((T + p.segment - 1) / p.segment) : 1;
     return p;
 }
-// waves of a workgroup: a tile of all of them if there are so many steps
+// waves of a workgroup: a tile of all of them if there are so many steps (the tiles of a loop then begin at kept states)
 int waves(int64_t steps) { return steps >= WAVES * STEPS ? WAVES : steps <= STEPS ? 1 : (int)((steps + STEPS - 1) / STEPS); }
 
-bool aligned(const void* p, int64_t st, int64_t sb, int vec, int bytes) {
-    return !p || (((uintptr_t)p % (vec * bytes)) == 0 && st % vec == 0 && sb % vec == 0);
-}
-template <int TYPE, int VEC, bool GATE, bool MASK> int launch(Scan S, bool back, hipStream_t s) {
+template <int TYPE, int VEC, bool GATE> int launch(Scan S, bool back, hipStream_t s) {
     const Split p = split(S.T, S.B * S.H, VEC);
     S.segment = p.segment; S.segments = p.segments;
-    const dim3 grid((unsigned)p.groups, p.segments);
-    const int nw = waves(S.T < p.segment ? S.T : p.segment);
+    S.masked = S.reset || S.lens;
+    // what a wave touches in a tile - STEPS steps of the sequences of 64 VEC channels, and of the one that the first of them begins inside - lies within 4 GB
+    const int64_t sequences = (64 * VEC + S.H - 1) / S.H, last = S.B - 1 < sequences ? S.B - 1 : sequences;
+    for (const Strides* st : {&S.sf, &S.sx, &S.so, &S.sy, &S.sdy, &S.sdf, &S.sdx, &S.sdo})
+        APX_REQUIRE((S.T <= 1 || st->t < ((int64_t)1 << 32)) && (last == 0 || st->b < ((int64_t)1 << 32)) &&
+                    (S.T <= 1 ? 0 : (STEPS - 1) * st->t) + last * (last ? st->b : 0) + 4ll * S.H < ((int64_t)1 << 32), "neighbouring steps or sequences lie too far apart");
+    APX_REQUIRE((STEPS - 1) * S.B + last < ((int64_t)1 << 32), "B");
+    const dim3 grid((unsigned)p.groups, p.segments), block(64 * waves(S.T < p.segment ? S.T : p.segment));
+    const size_t maps = block.x * VEC * sizeof(Map);      // LDS for one map a thread and channel
     if (p.segments > 1) {
-        if (back) hipLaunchKernelGGL((gated_scan_maps_kernel<TYPE, VEC, GATE, MASK, true>), grid, dim3(64 * nw), 0, s, S);
-        else hipLaunchKernelGGL((gated_scan_maps_kernel<TYPE, VEC, false, MASK, false>), grid, dim3(64 * nw), 0, s, S);
+        if (back) hipLaunchKernelGGL((gated_scan_maps_kernel<TYPE, VEC, GATE, true>), grid, block, maps, s, S);
+        else hipLaunchKernelGGL((gated_scan_maps_kernel<TYPE, VEC, false, false>), grid, block, maps, s, S);
         APX_LAUNCH_CHECK();
     }
-    if (back) hipLaunchKernelGGL((gated_scan_bwd_kernel<TYPE, VEC, GATE, MASK>), grid, dim3(64 * nw), 0, s, S);
-    else hipLaunchKernelGGL((gated_scan_fwd_kernel<TYPE, VEC, GATE, MASK>), grid, dim3(64 * nw), 0, s, S);
+    if (back) hipLaunchKernelGGL((gated_scan_bwd_kernel<TYPE, VEC, GATE>), grid, block, 3 * maps, s, S);
+    else hipLaunchKernelGGL((gated_scan_fwd_kernel<TYPE, VEC, GATE>), grid, block, 2 * maps, s, S);
     APX_LAUNCH_CHECK();
     return APX_OK;
 }
-template <int TYPE, int VEC> int by_masks(const Scan& S, bool back, hipStream_t s) {
-    const bool gate = S.o != nullptr, mask = S.reset || S.lens;
-    if (gate) return mask ? launch<TYPE, VEC, true, true>(S, back, s) : launch<TYPE, VEC, true, false>(S, back, s);
-    return mask ? launch<TYPE, VEC, false, true>(S, back, s) : launch<TYPE, VEC, false, false>(S, back, s);
+template <int TYPE> int by_width(const Scan& S, bool back, hipStream_t s) {
+    if (S.H % VECTOR == 0) return S.o ? launch<TYPE, VECTOR, true>(S, back, s) : launch<TYPE, VECTOR, false>(S, back, s);
+    return S.o ? launch<TYPE, 1, true>(S, back, s) : launch<TYPE, 1, false>(S, back, s);
 }
 int run(int type, Scan& S, bool back, void* workspace, hipStream_t s) {
     S.maps = (Map*)workspace;
-    const int bytes = type == APX_F32 ? 4 : 2;
-    bool wide = S.H % 2 == 0;
-    const void* p[7] = {S.f, S.x, S.o, back ? S.dy : S.y, back ? S.df : nullptr, back ? S.dx : nullptr, back && S.o ? S.do_ : nullptr};
-    const Strides* st[7] = {&S.sf, &S.sx, &S.so, back ? &S.sdy : &S.sy, &S.sdf, &S.sdx, &S.sdo};
-    for (int i = 0; i < 7; ++i) wide = wide && aligned(p[i], st[i]->t, st[i]->b, 2, bytes);
-    if (type == APX_F32) return wide ? by_masks<APX_F32, 2>(S, back, s) : by_masks<APX_F32, 1>(S, back, s);
-    if (type == APX_BF16) return wide ? by_masks<APX_BF16, 2>(S, back, s) : by_masks<APX_BF16, 1>(S, back, s);
-    return wide ? by_masks<APX_F16, 2>(S, back, s) : by_masks<APX_F16, 1>(S, back, s);
+    return type == APX_F32 ? by_width<APX_F32>(S, back, s) : type == APX_BF16 ? by_width<APX_BF16>(S, back, s) : by_width<APX_F16>(S, back, s);
 }
 
 }  // namespace
@@ -512,13 +660,8 @@ extern "C" size_t apx_gated_scan_save_floats(int64_t T, int64_t B, int H) {
 }
 extern "C" size_t apx_gated_scan_workspace_bytes(int64_t T, int64_t B, int H) {
     if (T <= 0 || B <= 0 || H <= 0) return 0;
-    size_t most = 0;
-    for (int vec = 1; vec <= 2; ++vec) {
-        const Split p = split(T, B * H, vec);
-        const size_t need = p.segments > 1 ? (size_t)p.segments * B * H * sizeof(Map) : 0;
-        if (need > most) most = need;
-    }
-    return most;
+    const Split p = split(T, B * H, H % VECTOR == 0 ? VECTOR : 1);
+    return p.segments > 1 ? (size_t)p.segments * B * H * sizeof(Map) : 0;
 }
 
 extern "C" int apx_gated_scan_forward(const apx_gated_scan_args* a, void* stream) {

@@ -17,4 +17,11 @@ __device__ __forceinline__ float sqrt_fast(float x) { return __builtin_amdgcn_sq
 // the value of the first lane, for what is the same in all lanes of a wave (a scalar register then)
 __device__ __forceinline__ int wave_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// an address in global memory that is the same in all lanes, kept in scalar registers (the compiler would rather add a lane's offset to it first and have 64-bit vector additions
+// from then on)
+#define APX_GLOBAL __attribute__((address_space(1)))
+template <class T> __device__ __forceinline__ APX_GLOBAL T* wave_address(T* p) { APX_GLOBAL T* q = (APX_GLOBAL T*)p; asm("" : "+s"(q)); return q; }
+// a lane's 32-bit offset, made where it is used (widened to 64 bits outside a loop it would take the vector additions again)
+__device__ __forceinline__ unsigned lane_offset(unsigned x) { asm("" : "+v"(x)); return x; }
+
 }  // namespace half_types

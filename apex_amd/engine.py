@@ -2,6 +2,7 @@
 torch.distributed.  Every function launches HIP kernels from libapx.so on the current torch stream."""
 import array
 import ctypes as C
+import operator
 import struct
 
 import numpy as np
@@ -16,7 +17,8 @@ def _p(t):
 
 
 def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current stream of the current device (its handle alone: the Stream object of torch.cuda.current_stream() costs 3 us of host time a call)."""
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def _need_gpu(*ts):
@@ -214,14 +216,18 @@ def _elsewhere(fn, dev, *a, **k):
 
 def _operand(name, t, like, dev, out=False):
     """(t, its three numbers in apx_gated_scan_args) for an operand [.., H] of f's shape, type and device; one whose units do not lie next to each other is copied (an output refused)"""
-    if t.shape != like.shape or t.dtype != like.dtype or t.get_device() != dev:
+    if t is not like and (t.shape != like.shape or t.dtype != like.dtype or t.get_device() != dev):
         raise ValueError("%s is %s %s on %s, expected %s %s on %s" % (name, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype, like.device))
     s = t.stride()
     if s[-1] != 1 and t.shape[-1] > 1:
         if out:
             raise ValueError("%s has stride %d along the units, expected 1" % (name, s[-1]))
         t = t.contiguous(); s = t.stride()
-    return t, (t.data_ptr(), s[0] if len(s) == 3 else 0, s[-2])
+    return t, ((t.data_ptr(), s[0], s[1]) if len(s) == 3 else (t.data_ptr(), 0, s[0]))
+
+
+def _like(f):
+    return torch.empty_like(f, memory_format=torch.contiguous_format)
 
 
 def _extra(name, t, shape, dtype, like, dev):
@@ -235,21 +241,21 @@ def _extra(name, t, shape, dtype, like, dev):
 
 
 _NONE = (0, 0, 0)
+_SHAPE, _DTYPE = operator.attrgetter("shape"), operator.attrgetter("dtype")
 
 
 def _scan_inputs(f, x, o, h0, reset, lens, dim=3):
     _need_gpu(f, x, o, h0, reset, lens)
-    if f.dim() != dim or f.dtype not in _TYPES:
-        raise ValueError("f is %s %s, expected [%sB, H] in f32, bf16 or f16" % (tuple(f.shape), f.dtype, "T, " if dim == 3 else ""))
+    shape, kind = f.shape, _TYPES.get(f.dtype)
+    if len(shape) != dim or kind is None:
+        raise ValueError("f is %s %s, expected [%sB, H] in f32, bf16 or f16" % (tuple(shape), f.dtype, "T, " if dim == 3 else ""))
     dev = f.get_device()
-    B, H = f.shape[-2:]
-    lead = tuple(f.shape[:-1])
+    T, B, H = shape if dim == 3 else (1, *shape)
     f, f3 = _operand("f", f, f, dev); x, x3 = _operand("x", x, f, dev); o, o3 = _operand("o", o, f, dev) if o is not None else (None, _NONE)
     h0, h0p = _extra("h0", h0, (B, H), torch.float32, f, dev)
-    reset, rp = _extra("reset", reset, lead, torch.uint8, f, dev)
+    reset, rp = _extra("reset", reset, (T, B) if dim == 3 else (B,), torch.uint8, f, dev)
     lens, lp = _extra("lens", lens, (B,), torch.int32, f, dev)
-    head = (_TYPES[f.dtype], H, f.shape[0] if dim == 3 else 1, B, *f3, *x3, *o3, h0p, rp, lp)
-    return head, dev, (f, x, o, h0, reset, lens)      # (the tensors that the numbers point into)
+    return (kind, H, T, B, *f3, *x3, *o3, h0p, rp, lp), dev, (f, x, o, h0, reset, lens)      # (the tensors that the numbers point into)
 
 
 def _scan_workspace(lib, T, B, H, like):
@@ -266,11 +272,11 @@ def gated_scan(f, x, o=None, h0=None, reset=None, lens=None, keep=False, out=Non
     from a zero state (an episode start); lens [B] int32: steps from lens[b] on are padding - the state stays and y is 0 there.  out: where y goes (it must not lie on an input).
     Returns (y [T, B, H], h_last [B, H] f32), with keep=True (y, h_last, save) for gated_scan_backward.  States, gates and sums are f32 whatever the type."""
     head, dev, held = _scan_inputs(f, x, o, h0, reset, lens)
-    if dev >= 0 and dev != torch.cuda.current_device():
+    if dev >= 0 and dev != torch._C._cuda_getDevice():
         return _elsewhere(gated_scan, dev, f, x, o, h0, reset, lens, keep, out)
     lib = _lib.load()
     _, H, T, B = head[:4]
-    y, y3 = _operand("out", torch.empty(f.shape, dtype=f.dtype, device=f.device) if out is None else out, f, dev, True)
+    y, y3 = _operand("out", _like(f) if out is None else out, f, dev, True)
     h_last = torch.empty(B, H, dtype=torch.float32, device=f.device)
     save = torch.empty(lib.apx_gated_scan_save_floats(T, B, H), dtype=torch.float32, device=f.device) if keep else None
     ws, wp, wn = _scan_workspace(lib, T, B, H, f)
@@ -284,7 +290,7 @@ def gated_scan_backward(f, x, dy, save, o=None, h0=None, reset=None, lens=None, 
     without h0.  out: (df, dx) or (df, dx, do) to write into - slices of one gradient of the product that made f | x | o, for instance."""
     head, dev, held = _scan_inputs(f, x, o, h0, reset, lens)
     _need_gpu(dy, save, dh_last)
-    if dev >= 0 and dev != torch.cuda.current_device():
+    if dev >= 0 and dev != torch._C._cuda_getDevice():
         return _elsewhere(gated_scan_backward, dev, f, x, dy, save, o, h0, reset, lens, dh_last, out)
     lib = _lib.load()
     _, H, T, B = head[:4]
@@ -295,7 +301,7 @@ def gated_scan_backward(f, x, dy, save, o=None, h0=None, reset=None, lens=None, 
     dh_last, dhp = _extra("dh_last", dh_last, (B, H), torch.float32, f, dev)
     k = 2 if o is None else 3
     if out is None:
-        out = [torch.empty(f.shape, dtype=f.dtype, device=f.device) for _ in range(k)]
+        out = [_like(f) for _ in range(k)]
     elif len(out) != k:
         raise ValueError("out holds %d tensors, expected %d" % (len(out), k))
     df, df3 = _operand("df", out[0], f, dev, True); dx, dx3 = _operand("dx", out[1], f, dev, True)
@@ -312,11 +318,11 @@ def gated_scan_step(f, x, h, o=None, reset=None, out=None):
     returns y [B, H]."""
     head, dev, held = _scan_inputs(f, x, o, None, reset, None, 2)
     _need_gpu(h)
-    if dev >= 0 and dev != torch.cuda.current_device():
+    if dev >= 0 and dev != torch._C._cuda_getDevice():
         return _elsewhere(gated_scan_step, dev, f, x, h, o, reset, out)
     if h.shape != f.shape or h.dtype != torch.float32 or h.get_device() != dev or not h.is_contiguous():
         raise ValueError("h is %s %s on %s, expected a dense %s f32 on %s" % (tuple(h.shape), h.dtype, h.device, tuple(f.shape), f.device))
-    y, y3 = _operand("out", torch.empty(f.shape, dtype=f.dtype, device=f.device) if out is None else out, f, dev, True)
+    y, y3 = _operand("out", _like(f) if out is None else out, f, dev, True)
     a = _lib.GatedScanArgs.from_buffer_copy(_SCAN_ARGS.pack(*head, *y3, 0, 0, *_NONE, 0, *_NONE, *_NONE, *_NONE, 0, 0, 0))
     check(_lib.load().apx_gated_scan_step(C.byref(a), C.c_void_p(h.data_ptr()), _stream()))
     return y
@@ -376,21 +382,20 @@ class AdamW:
         n, index = len(self.params), self._index
         if len(grads) != n:
             raise ValueError("%d gradients for %d tensors" % (len(grads), n))
-        _need_gpu(*grads)
         kind = grads[0].dtype
         if kind not in _TYPES:
             raise ValueError("gradients in %s: f32, bf16 and f16 are served" % (kind,))
-        if ([g.shape for g in grads] != self._shapes or any([g.dtype != kind for g in grads]) or any([g.get_device() != index for g in grads])
-                or not all([g.is_contiguous() for g in grads])):
+        # (map over the methods themselves: with hundreds of small tensors these checks are what a step takes)
+        if (list(map(_SHAPE, grads)) != self._shapes or set(map(_DTYPE, grads)) != {kind} or set(map(torch.Tensor.get_device, grads)) != {index}
+                or not all(map(torch.Tensor.is_contiguous, grads))):
             for i, (g, p) in enumerate(zip(grads, self.params)):
                 if g.dtype != kind or g.device != self.device or g.shape != p.shape or not g.is_contiguous():
                     raise ValueError("grads[%d] is %s %s on %s, expected a dense %s %s on %s" % (i, tuple(g.shape), g.dtype, g.device, tuple(p.shape), kind, self.device))
-        at = [p.data_ptr() for p in self.params]
-        if at != self._pointers:
+        if list(map(torch.Tensor.data_ptr, self.params)) != self._pointers:
             raise ValueError("a tensor of params has moved since this optimiser was made: it works on the memory that it was given")
-        if index >= 0 and index != torch.cuda.current_device():
+        if index >= 0 and index != torch._C._cuda_getDevice():
             return _elsewhere(self.step, index, grads, grad_scale, lr)
-        gs = array.array("Q", [g.data_ptr() for g in grads])
+        gs = array.array("Q", map(torch.Tensor.data_ptr, grads))
         a = self._args
         a.grad_type, a.grads, a.lr, a.grad_scale = _TYPES[kind], gs.buffer_info()[0], self.lr if lr is None else lr, grad_scale
         a.beta1, a.beta2, a.eps, a.max_norm, a.seed = *self.betas, self.eps, 0.0 if self.max_norm is None else self.max_norm, self.seed

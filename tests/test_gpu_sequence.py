@@ -24,7 +24,8 @@ SCANS = [
     dict(T=63, B=7, H=130, gate=True), dict(T=64, B=7, H=130, t="bf16"), dict(T=65, B=7, H=130, reset=True), dict(T=127, B=2, H=66, t="bf16", gate=True, carry=True), dict(T=129, B=2, H=72, carry=True),
     dict(T=255, B=1, H=256, reset=True), dict(T=257, B=1, H=256, t="bf16", gate=True, lens=True), dict(T=1000, B=1, H=128, carry=True), dict(T=1025, B=3, H=24, reset=True, gate=True, carry=True),
     dict(T=4099, B=1, H=128, reset=True, carry=True, lean=4.0), dict(T=5000, B=2, H=8, t="bf16", gate=True, lens=True, carry=True), dict(T=3001, B=1, H=5, t="f16", gate=True, reset=True),
-    dict(T=2048, B=5, H=100, lens=True, carry=True), dict(T=12345, B=1, H=2, gate=True, lean=5.0),
+    dict(T=2048, B=5, H=100, lens=True, carry=True), dict(T=12345, B=1, H=2, gate=True, lean=5.0), dict(T=70001, B=1, H=6, reset=True, carry=True, lean=5.0), dict(T=16448, B=2, H=33, t="bf16", gate=True, lens=True, carry=True),
+    dict(T=512, B=1, H=4, carry=True), dict(T=513, B=1, H=4, carry=True), dict(T=575, B=60, H=130, gate=True, reset=True), dict(T=640, B=250, H=128, t="f16"), dict(T=511, B=1, H=4, lens=True),
     dict(T=70, B=33, H=16, gate=True, lens=True, layout="batch first"), dict(T=600, B=2, H=64, t="bf16", reset=True, carry=True, layout="batch first"),
     dict(T=90, B=9, H=64, gate=True, carry=True, layout="shifted"), dict(T=90, B=9, H=64, t="bf16", reset=True, layout="shifted"), dict(T=2100, B=1, H=64, t="f16", carry=True, layout="shifted"),
     dict(T=90, B=9, H=64, gate=True, carry=True, layout="dense"), dict(T=600, B=3, H=60, t="bf16", layout="dense"),

@@ -13,7 +13,8 @@ SCANS = [
     dict(T=1, B=1, H=1), dict(T=1, B=3, H=5, gate=True, reset=True, lens=True, carry=True), dict(T=7, B=2, H=3, carry=True), dict(T=16, B=1, H=64, gate=True),
     dict(T=17, B=3, H=21, reset=True, carry=True), dict(T=33, B=2, H=40, t="bf16", gate=True, lens=True, carry=True), dict(T=50, B=3, H=17, t="f16", reset=True, lens=True, carry=True),
     dict(T=40, B=5, H=13, gate=True, reset=True, lens=True, carry=True, poison=True), dict(T=300, B=1, H=8, reset=True, carry=True, lean=4.0), dict(T=130, B=1, H=65, t="bf16", gate=True),
-    dict(T=70, B=2, H=16, gate=True, lens=True, layout="batch first"), dict(T=20, B=2, H=12, gate=True, carry=True, layout="shifted"), dict(T=21, B=2, H=12, t="bf16", layout="dense"),
+    dict(T=600, B=2, H=10, reset=True, carry=True), dict(T=1100, B=1, H=3, gate=True, lens=True, carry=True, t="bf16"), dict(T=17000, B=1, H=1, reset=True, carry=True, lean=4.0),
+    dict(T=1030, B=3, H=44, gate=True, reset=True, lens=True, carry=True, poison=True, t="f16"), dict(T=70, B=2, H=16, gate=True, lens=True, layout="batch first"), dict(T=20, B=2, H=12, gate=True, carry=True, layout="shifted"), dict(T=21, B=2, H=12, t="bf16", layout="dense"),
 ]
 
 

@@ -35,5 +35,8 @@ inline float rcp_fast(float x) { return 1.0f / x; }
 inline float sqrt_fast(float x) { return sqrtf(x); }
 
 inline int wave_uniform(int x) { return x; }
+inline unsigned lane_offset(unsigned x) { return x; }
+#define APX_GLOBAL
+template <class T> inline T* wave_address(T* p) { return p; }
 
 }  // namespace half_types
