@@ -18,8 +18,8 @@ constexpr int TABLE = 120;                 // entries a launch: 32 bytes each, o
 constexpr int BLOCK = 256;                 // elements that share a scale of 8-bit moments, and what a tensor's part of the moments is rounded up to
 constexpr int CHUNK = 2048;                // elements a workgroup takes at a time: 8 blocks, 8 elements a thread
 constexpr int64_t ENTRY = (int64_t)1 << 31;      // elements of an entry: a larger tensor takes several
-constexpr int PARTS = 1024;                // partial sums of squares of one launch
-constexpr int GRID = 2048;                 // workgroups of the update at most: 8 for each of 256 CUs
+constexpr int PARTS = 1024;               // partial sums of squares of one launch
+constexpr int GRID = 4096;                 // workgroups of the update at most: 16 for each of 256 CUs (8 were 4 % slower)
 constexpr unsigned M_OFFSET = 904, V_OFFSET = 776;
 
 struct Table {
@@ -41,17 +41,20 @@ __device__ __forceinline__ int entry_of(const Table& T, int chunk) {
     return lo;
 }
 // 4 elements by one wide access, on any boundary that their type allows (tensors are views at any offset of a flat block)
-struct alignas(4) F4 { float v[4]; };
-struct alignas(2) H4 { uint16_t v[4]; };
+typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t H4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t C4 __attribute__((aligned(4)));      // 4 codes
+// Parameters and moments pass by the caches (nobody reads them again soon, and 63 M parameters' 750 MB would drive out the gradients, which the norm has just brought into the
+// 256 MB before the memory: the update of such a network took 320 us with ordinary accesses and takes 268)
 template <int TYPE> __device__ __forceinline__ void load_grad(const void* g, int64_t i, float (&o)[4]) {
     if constexpr (TYPE == APX_F32) {
         const F4 r = *(const F4*)((const float*)g + i);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = r.v[k];
+        for (int k = 0; k < 4; ++k) o[k] = r[k];
     } else {
         const H4 r = *(const H4*)((const uint16_t*)g + i);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = TYPE == APX_BF16 ? widen_bf16(r.v[k]) : widen_f16(r.v[k]);
+        for (int k = 0; k < 4; ++k) o[k] = TYPE == APX_BF16 ? widen_bf16(r[k]) : widen_f16(r[k]);
     }
 }
 template <int TYPE> __device__ __forceinline__ float grad_at(const void* g, int64_t i) {
@@ -143,14 +146,18 @@ __global__ __launch_bounds__(256) void adamw32_kernel(Table T, Hyper P, float* _
             for (int q = 0; q < 2; ++q) {
                 const int i = q * 1024 + threadIdx.x * 4;
                 load_grad<TYPE>(T.g[id], (int64_t)e0 + i, g[q]);
-                pp[q] = *(const F4*)(p + i); mm[q] = *(const F4*)(m + i); vv[q] = *(const F4*)(v + i);
+                pp[q] = APX_PASSING((const F4*)(p + i)); mm[q] = APX_PASSING((const F4*)(m + i)); vv[q] = APX_PASSING((const F4*)(v + i));
             }
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 const int i = q * 1024 + threadIdx.x * 4;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) adam(g[q][k] * c, mm[q].v[k], vv[q].v[k], pp[q].v[k], P, S, keep);
-                *(F4*)(p + i) = pp[q]; *(F4*)(m + i) = mm[q]; *(F4*)(v + i) = vv[q];
+                for (int k = 0; k < 4; ++k) {
+                    float x = pp[q][k], y = mm[q][k], z = vv[q][k];
+                    adam(g[q][k] * c, y, z, x, P, S, keep);
+                    pp[q][k] = x; mm[q][k] = y; vv[q][k] = z;
+                }
+                APX_PASS((F4*)(p + i), pp[q]); APX_PASS((F4*)(m + i), mm[q]); APX_PASS((F4*)(v + i), vv[q]);
             }
         } else {
             for (unsigned i = threadIdx.x; i < left; i += 256) adam(grad_at<TYPE>(T.g[id], (int64_t)e0 + i) * c, m[i], v[i], p[i], P, S, keep);
@@ -209,7 +216,6 @@ __device__ __forceinline__ unsigned wave_top(unsigned x) {
     for (int row = 16; row < 64; row += 16) { const unsigned y = (unsigned)__builtin_amdgcn_readlane((int)x, row); r = r > y ? r : y; }
     return r;
 }
-struct alignas(4) Code4 { uint8_t v[4]; };
 
 // A wave takes a block of 256 elements at a time, a lane 4 of them, two blocks of a chunk at once so that twice as many loads are on their way.  Codes and scales are exact in
 // f32 (scales are powers of two), the block's largest is found on the bits, so the same inputs give the same codes whatever the launch looks like.
@@ -225,20 +231,20 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Table T, Hyper P, uint8_t* 
         const float keep = 1.f - P.lr * T.wd[id];
         const unsigned n = T.n[id], e0 = (unsigned)(chunk - T.first[id]) * CHUNK;
         float* const p = T.p[id];
-        float g[2][4], ms[2], vs[2]; F4 pp[2]; Code4 mm[2], vv[2];
+        float g[2][4], ms[2], vs[2]; F4 pp[2]; C4 mm[2], vv[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const unsigned e = e0 + (q * 4 + wave) * BLOCK;
             if (e >= n) continue;
             const int64_t blk = (int64_t)T.state[id] + e / BLOCK;
             const unsigned i = e + lane * 4;
-            if (n - e >= BLOCK) { load_grad<TYPE>(T.g[id], i, g[q]); pp[q] = *(const F4*)(p + i); }
+            if (n - e >= BLOCK) { load_grad<TYPE>(T.g[id], i, g[q]); pp[q] = APX_PASSING((const F4*)(p + i)); }
             else {
                 load_grad_end<TYPE>(T.g[id], i, (int)(n - e) - lane * 4, g[q]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) pp[q].v[k] = i + k < n ? p[i + k] : 0.f;
+                for (int k = 0; k < 4; ++k) pp[q][k] = i + k < n ? p[i + k] : 0.f;
             }
-            mm[q] = *(const Code4*)(M + blk * BLOCK + lane * 4); vv[q] = *(const Code4*)(V + blk * BLOCK + lane * 4);
+            mm[q] = APX_PASSING((const C4*)(M + blk * BLOCK + lane * 4)); vv[q] = APX_PASSING((const C4*)(V + blk * BLOCK + lane * 4));
             ms[q] = MS[blk]; vs[q] = VS[blk];
         }
 #pragma unroll
@@ -251,26 +257,28 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Table T, Hyper P, uint8_t* 
             unsigned mt = 0, vt = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {      // (behind the tensor's end: codes, gradient and parameter 0 stay 0)
-                m[k] = decode_m(mm[q].v[k], ms[q]); v[k] = decode_v(vv[q].v[k], vs[q]);
-                adam(g[q][k] * c, m[k], v[k], pp[q].v[k], P, S, keep);
+                m[k] = decode_m(mm[q] >> 8 * k & 255u, ms[q]); v[k] = decode_v(vv[q] >> 8 * k & 255u, vs[q]);
+                float x = pp[q][k];
+                adam(g[q][k] * c, m[k], v[k], x, P, S, keep);
+                pp[q][k] = x;
                 if (n - e < BLOCK && i + k >= n) m[k] = v[k] = 0.f;      // (0 times an infinite scale factor, say)
                 const unsigned am = __float_as_uint(m[k]) & 0x7fffffffu, av = __float_as_uint(v[k]) & 0x7fffffffu;      // (as integers: a NaN is larger than all numbers)
                 mt = mt > am ? mt : am; vt = vt > av ? vt : av;
             }
-            if (n - e >= BLOCK) *(F4*)(p + i) = pp[q];
+            if (n - e >= BLOCK) APX_PASS((F4*)(p + i), pp[q]);
             else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) if (i + k < n) p[i + k] = pp[q].v[k];
+                for (int k = 0; k < 4; ++k) if (i + k < n) p[i + k] = pp[q][k];
             }
             float s, inv, s2, inv2;
             block_scale(wave_top(mt), s, inv); block_scale(wave_top(vt), s2, inv2);
-            Code4 mo, vo;
+            C4 mo = 0, vo = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const unsigned r = element_noise(key, blk * BLOCK + lane * 4 + k);
-                mo.v[k] = (uint8_t)encode_m(m[k], inv, r & 0xffffu); vo.v[k] = (uint8_t)encode_v(v[k], inv2, r >> 16);
+                mo |= (encode_m(m[k], inv, r & 0xffffu) & 255u) << 8 * k; vo |= (encode_v(v[k], inv2, r >> 16) & 255u) << 8 * k;
             }
-            *(Code4*)(M + blk * BLOCK + lane * 4) = mo; *(Code4*)(V + blk * BLOCK + lane * 4) = vo;
+            APX_PASS((C4*)(M + blk * BLOCK + lane * 4), mo); APX_PASS((C4*)(V + blk * BLOCK + lane * 4), vo);
             if (lane == 0) { MS[blk] = s; VS[blk] = s2; }
         }
     }

@@ -14,6 +14,9 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }        // v_rcp_f32: 1 ulp
 __device__ __forceinline__ float sqrt_fast(float x) { return __builtin_amdgcn_sqrtf(x); }      // v_sqrt_f32: 1 ulp
 
+// accesses that leave the caches to others (macros: a template parameter would lose the alignment of the pointer's type)
+#define APX_PASSING(p) __builtin_nontemporal_load(p)
+#define APX_PASS(p, x) __builtin_nontemporal_store(x, p)
 // the value of the first lane, for what is the same in all lanes of a wave (a scalar register then)
 __device__ __forceinline__ int wave_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 

@@ -34,6 +34,8 @@ inline float exp2_fast(float x) { return exp2f(x); }
 inline float rcp_fast(float x) { return 1.0f / x; }
 inline float sqrt_fast(float x) { return sqrtf(x); }
 
+#define APX_PASSING(p) (*(p))
+#define APX_PASS(p, x) (*(p) = (x))
 inline int wave_uniform(int x) { return x; }
 inline unsigned lane_offset(unsigned x) { return x; }
 #define APX_GLOBAL
