@@ -337,6 +337,7 @@ extern "C" int apx_adamw(const apx_adamw_args* a, void* stream) {
     for (int i = 0; i < a->n_tensors; ++i) {
         APX_REQUIRE(a->numel[i] >= 0 && a->numel[i] < ((int64_t)1 << 39), "numel");
         APX_REQUIRE(a->numel[i] == 0 || (a->params[i] && a->grads[i]), "null tensor");
+        APX_REQUIRE(!a->weight_decay || std::isfinite(a->weight_decay[i]), "weight_decay");
         total += a->numel[i];
     }
     APX_REQUIRE(total < ((int64_t)1 << 39), "numel in all");

@@ -618,8 +618,8 @@ template <int TYPE, int VEC, bool GATE> int launch(Scan S, bool back, hipStream_
     const Split p = split(S.T, S.B * S.H, VEC);
     S.segment = p.segment; S.segments = p.segments;
     S.masked = S.reset || S.lens;
-    // what a wave touches in a tile - STEPS steps of the sequences of 64 VEC channels, and of the one that the first of them begins inside - lies within 4 GB
-    const int64_t sequences = (64 * VEC + S.H - 1) / S.H, last = S.B - 1 < sequences ? S.B - 1 : sequences;
+    // what a wave touches in a tile - STEPS steps of the sequences that its 64 VEC channels belong to - lies within 4 GB; `last`: how many sequences behind its first one
+    const int64_t n = 64 * VEC, more = S.H % n == 0 ? 0 : n % S.H == 0 ? n / S.H - 1 : n / S.H + 1, last = S.B - 1 < more ? S.B - 1 : more;
     for (const Strides* st : {&S.sf, &S.sx, &S.so, &S.sy, &S.sdy, &S.sdf, &S.sdx, &S.sdo})
         APX_REQUIRE((S.T <= 1 || st->t < ((int64_t)1 << 32)) && (last == 0 || st->b < ((int64_t)1 << 32)) &&
                     (S.T <= 1 ? 0 : (STEPS - 1) * st->t) + last * (last ? st->b : 0) + 4ll * S.H < ((int64_t)1 << 32), "neighbouring steps or sequences lie too far apart");

@@ -344,13 +344,16 @@ class AdamW:
         for i, p in enumerate(self.params):
             if p.dtype != torch.float32 or p.device != self.device or not p.is_contiguous():
                 raise ValueError("params[%d] is %s on %s%s, expected a dense f32 tensor on %s" % (i, p.dtype, p.device, "" if p.is_contiguous() else " with gaps", self.device))
+        spans = sorted((p.data_ptr(), p.data_ptr() + 4 * p.numel()) for p in self.params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("two tensors of params overlap (or one is given twice): a step would update the same memory twice")
         if state_bits not in (8, 32):
             raise ValueError("state_bits is 8 or 32, not %r" % (state_bits,))
         n = len(self.params)
         decay = [float(weight_decay)] * n if not isinstance(weight_decay, (list, tuple)) else [float(w) for w in weight_decay]
         if len(decay) != n:
             raise ValueError("%d weight decays for %d tensors" % (len(decay), n))
-        self.lr, self.betas, self.eps, self.max_norm, self.state_bits, self.seed = lr, betas, eps, max_norm, state_bits, int(seed)
+        self.lr, self.betas, self.eps, self.max_norm, self.state_bits, self.seed = lr, betas, eps, max_norm, state_bits, int(seed) & (1 << 64) - 1
         lib = _lib.load()
         self._numel = (C.c_int64 * n)(*[p.numel() for p in self.params])
         self._decay = (C.c_float * n)(*decay)
@@ -367,7 +370,7 @@ class AdamW:
         self._index, self._shapes = self.params[0].get_device(), [p.shape for p in self.params]
         self._held = [p.detach() for p in self.params]      # (keeps the memory that the pointers below name)
         self._pointers = [p.data_ptr() for p in self.params]
-        self._ps = array.array("Q", self._pointers)
+        self._ps, self._taken = array.array("Q", self._pointers), {p.data_ptr() for p in self.params if p.numel()}
         self._args = _lib.AdamwArgs(n_tensors=n, state_bits=state_bits, params=self._ps.buffer_info()[0], numel=C.addressof(self._numel), weight_decay=C.addressof(self._decay),
                                     m=_p(self.m), v=_p(self.v), m_scale=_p(self.m_scale), v_scale=_p(self.v_scale), t=_p(self.t), workspace=_p(self._ws),
                                     workspace_bytes=self._ws.numel(), norm_out=_p(self.norm))
@@ -396,6 +399,10 @@ class AdamW:
         if index >= 0 and index != torch._C._cuda_getDevice():
             return _elsewhere(self.step, index, grads, grad_scale, lr)
         gs = array.array("Q", map(torch.Tensor.data_ptr, grads))
+        if not self._taken.isdisjoint(gs):
+            raise ValueError("a gradient lies on a tensor of params")
+        if self.max_norm is not None and not self.max_norm > 0:
+            raise ValueError("max_norm is %r, expected a positive number or None" % (self.max_norm,))
         a = self._args
         a.grad_type, a.grads, a.lr, a.grad_scale = _TYPES[kind], gs.buffer_info()[0], self.lr if lr is None else lr, grad_scale
         a.beta1, a.beta2, a.eps, a.max_norm, a.seed = *self.betas, self.eps, 0.0 if self.max_norm is None else self.max_norm, self.seed

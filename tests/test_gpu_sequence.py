@@ -148,6 +148,18 @@ def test_long_offsets(dev):
     del y2
 
 
+def test_long_offsets_batch_first(dev):
+    """sequences of 1.1 x 10^9 elements each, one behind the other in memory: steps and sequences beyond 2^31 elements, against a scan of the last rows alone"""
+    from apex_amd import engine
+    T, B, H, K = 9000000, 3, 128, 70
+    f = torch.empty(B, T, H, dtype=torch.bfloat16, device=dev).normal_().permute(1, 0, 2)
+    out = torch.empty(B, T, H, dtype=torch.bfloat16, device=dev).permute(1, 0, 2)
+    reset = torch.zeros(T, B, dtype=torch.uint8, device=dev); reset[T - K] = 1
+    y, h = engine.gated_scan(f, f, reset=reset, out=out)
+    ys, hs = engine.gated_scan(f[T - K:], f[T - K:])
+    assert (y[T - K:].float() - ys.float()).abs().max() <= 2 ** -7 * ys.float().abs().max() and (h - hs).abs().max() <= 1e-5
+
+
 def test_rows_outside_the_outputs_stay(dev):
     """outputs written into slices of larger buffers leave everything around them as it was"""
     from apex_amd import engine
@@ -198,6 +210,21 @@ ADAMW = [
 @pytest.mark.parametrize("case", ADAMW, ids=lambda c: "%d-%s-%s" % (len(c["shapes"]), c.get("bits", 32), c.get("grad", "f32")))
 def test_adamw_against_64_bits(dev, case):
     S.check_adamw(dev, **case)
+
+
+def test_adamw_a_tensor_beyond_32_bits(dev):
+    """2^31 + 5000 elements in one tensor: around the 2^31st and at the end what a small optimiser makes of the same elements"""
+    from apex_amd import engine
+    n = 2 ** 31 + 5000
+    p = torch.empty(n, device=dev).normal_(); g = torch.empty(n, dtype=torch.bfloat16, device=dev).normal_()
+    cuts = [slice(0, 300), slice(2 ** 31 - 2500, 2 ** 31 + 2500), slice(n - 300, n)]
+    small = [p[c].clone() for c in cuts]
+    o, e = engine.AdamW([p, torch.zeros(3, device=dev)], weight_decay=0.1), engine.AdamW(small, weight_decay=0.1)
+    for _ in range(2):
+        o.step([g, torch.ones(3, dtype=torch.bfloat16, device=dev)])
+        e.step([g[c].contiguous() for c in cuts])
+    for c, q, m in zip(cuts, small, e.views(e.m)):
+        assert torch.equal(p[c], q) and torch.equal(o.m[c], m)
 
 
 def test_adamw_stands_for_clip_adam(dev):

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import sequence as Q
 from tests import sequence_bodies as S
 from tests.test_kernel_emulation_learner import dev  # noqa: F401  (the fixture that puts the emulated library in place)
 
@@ -39,6 +40,19 @@ def test_emulated_scan_of_nothing(dev):  # noqa: F811
     assert torch.equal(h, h0[:2]) and not y.any()
     a, b = engine.gated_scan(f, f), engine.gated_scan(f, f, lens=torch.tensor([6, 2 ** 31 - 1], dtype=torch.int32))
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_emulated_scan_reset_everywhere(dev):  # noqa: F811
+    """a reset in front of every step: no step sees another one, whatever the start"""
+    from apex_amd import engine
+    for T in (5, 300):
+        f, x, r = torch.randn(T, 2, 6), torch.randn(T, 2, 6), torch.ones(T, 2, dtype=torch.uint8)
+        y, h, save = engine.gated_scan(f, x, h0=torch.full((2, 6), float("nan")), reset=r, keep=True)
+        want = Q.sigmoid(-S.f64(f)) * S.f64(x)
+        assert np.abs(S.f64(y) - want).max() < 1e-6 * np.abs(want).max() and torch.equal(h, y[-1])
+        df, dx, _, dh0 = engine.gated_scan_backward(f, x, torch.ones(T, 2, 6), save, h0=torch.zeros(2, 6), reset=r, dh_last=torch.zeros(2, 6))
+        a, n = Q.sigmoid(S.f64(f)), Q.sigmoid(-S.f64(f))
+        assert np.abs(S.f64(dx) - n).max() < 1e-6 and np.abs(S.f64(df) + S.f64(x) * a * n).max() < 1e-6 * 4 and not dh0.any()
 
 
 @pytest.mark.parametrize("case", [dict(B=1, H=1), dict(B=5, H=13, gate=True, reset=True), dict(B=3, H=64, t="bf16", gate=True), dict(B=4, H=8, t="f16", reset=True),
@@ -108,13 +122,15 @@ def test_refusals_of_the_wrappers(dev):  # noqa: F811
             lambda: engine.gated_scan_backward(f, x, x, save, out=(torch.zeros(4, 2, 3),)), lambda: engine.gated_scan_backward(f, x, x, save, dh_last=torch.zeros(3, 2))]
     t = torch.zeros(4, 2, 3)
     bad += [lambda: engine.gated_scan_backward(f, x, x, save, out=(t, t)), lambda: engine.gated_scan_backward(f, x, torch.ones(4, 2, 3), save, out=(t, f))]
-    p = [torch.zeros(3), torch.zeros(4)]
+    p, q = [torch.zeros(3), torch.zeros(4)], torch.zeros(9)
     bad += [lambda: engine.AdamW([]), lambda: engine.AdamW([torch.zeros(3).double()]), lambda: engine.AdamW([torch.zeros(3, 4).t()]), lambda: engine.AdamW(p, state_bits=16),
-            lambda: engine.AdamW(p, weight_decay=[0.1])]
+            lambda: engine.AdamW(p, weight_decay=[0.1]), lambda: engine.AdamW([p[0], p[0]]), lambda: engine.AdamW([q[:5], q[4:]])]
     o = engine.AdamW(p)
     bad += [lambda: o.step([torch.zeros(3)]), lambda: o.step([torch.zeros(3), torch.zeros(5)]), lambda: o.step([torch.zeros(3), torch.zeros(4).bfloat16()]),
             lambda: o.step([torch.zeros(3).double(), torch.zeros(4).double()]), lambda: o.step([torch.zeros(6)[::2], torch.zeros(4)]),
             lambda: engine.AdamW(p, eps=0.0).step([torch.zeros(3), torch.zeros(4)]), lambda: engine.AdamW(p, betas=(1.0, 0.9)).step([torch.zeros(3), torch.zeros(4)]),
+            lambda: engine.AdamW(p, max_norm=0.0).step([torch.zeros(3), torch.zeros(4)]), lambda: engine.AdamW(p, max_norm=-1.0).step([torch.zeros(3), torch.zeros(4)]),
+            lambda: o.step([p[0], torch.zeros(4)]), lambda: engine.AdamW(p, weight_decay=float("nan")).step([torch.zeros(3), torch.zeros(4)]),
             lambda: engine.AdamW(p, lr=float("nan")).step([torch.zeros(3), torch.zeros(4)])]
     for i, call in enumerate(bad):
         with pytest.raises((ValueError, RuntimeError)):
@@ -138,7 +154,7 @@ def test_refusals_of_the_c_entry_points():
     F, Bk = lib.apx_gated_scan_forward, lib.apx_gated_scan_backward
     calls = [scan(F, type=3), scan(F, type=-1), scan(F, T=-1), scan(F, B=-1), scan(F, H=-1), scan(F, f=None), scan(F, x=None), scan(F, y=None), scan(F, h_last=None),
              scan(F, f_t=-8), scan(F, y_b=3), scan(F, y_t=7), scan(F, y_t=0), scan(F, y=one), scan(F, h0=4 * one), scan(F, o=9 * one, o_t=-1), scan(F, T=1 << 58), scan(F, B=1 << 35),
-             scan(F, f_t=1 << 60), scan(Bk, save=None), scan(Bk, dy=None), scan(Bk, df=7 * one), scan(Bk, df=one), scan(Bk, o=9 * one, o_t=8, o_b=4), scan(Bk, dx_b=0),
+             scan(F, f_t=1 << 60), scan(F, f_t=1 << 30), scan(F, x_b=1 << 30), scan(Bk, dy_b=1 << 31), scan(Bk, save=None), scan(Bk, dy=None), scan(Bk, df=7 * one), scan(Bk, df=one), scan(Bk, o=9 * one, o_t=8, o_b=4), scan(Bk, dx_b=0),
              scan(Bk, dh0=11 * one, dh_last=11 * one)]
     s = _lib.GatedScanArgs(type=0, H=4, B=2, f=one, f_b=4, x=2 * one, x_b=4, y=3 * one, y_b=4)
     calls.append(lib.apx_gated_scan_step(C.byref(s), None, None))
