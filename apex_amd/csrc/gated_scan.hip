@@ -4,8 +4,15 @@
 //   backward, c_{T-1} = dh_last:  g_t = dy_t sigmoid(o_t) + c_t;   c_{t-1} = reset ? 0 : a_t g_t;   dh0 = c_{-1}
 //     dx_t = n_t g_t     df_t = g_t (p_t - x_t) a_t n_t     do_t = dy_t h_t s (1 - s), s = sigmoid(o_t)
 //
-// The channels (b, j) are independent of each other.  The backward pass needs every h_t again: the forward pass keeps the state in front of every 32nd step (f32), and the steps
-// between are run again from there.
+// The channels (b, j) are independent of each other.  The backward pass needs every h_t again: the forward pass keeps the state in front of every 32nd step (f32, 1/32 of the
+// states), and the steps between are run again from there.
+//
+// What bounds it: memory.  Forward f, x (o) in, y out; backward f, x, dy (o) in, df, dx (do) out: 3 to 7 elements moved for some 45 to 90 vector instructions, so f32 runs at the
+// rate of a copy (5.0 TB/s on this card) and 16-bit types are near the rate at which the vector units issue.  Measured on an MI355X, kernel times:
+//   forward  f32  [400, 1024, 128], resets            124 us   5.1 TB/s        bf16 [32, 4096, 256], resets             39 us   5.2 TB/s
+//   backward f32  [400, 1024, 128], output gate       305 us   4.8 TB/s        bf16 [32, 4096, 256], resets             79 us   4.2 TB/s
+//   the same f32 pair with lengths of 1 .. 400 (half of the rows are padding and are not read): forward 129 us, backward 246 us
+//   forward  bf16 [16384, 4, 256], output gate: maps 15 us + scan 26 us; f32 [65536, 1, 128]: maps 13 + 20 us, backward maps 13 + 29 us (the split reads f and x or dy twice)
 #include "apx_common.h"
 #include <gfx950/dynamic_lds.h>
 #include <gfx950/half_types.h>
@@ -35,21 +42,31 @@ template <> struct Elem<APX_F16> {
 constexpr int STEPS = 8;                  // steps of a wave in a tile: they stay in its registers
 constexpr int WAVES = 8;                  // waves of a workgroup at most
 constexpr int KEEP = 32;                  // steps between two kept states; what a tile begins with is one of them
-constexpr int VECTOR = 2;                 // channels of a lane, where H is even
-constexpr int SEGMENTS = 256;             // parts of the time axis at most
-constexpr int SPLIT = 128;                // steps that are worth a split at least
-constexpr int FILL = 512;                 // workgroups that fill the chip
+// Channels of a lane: 2 where H is even (no pair lies across two sequences then).  One channel: bf16 [32, 4096, 256] forward 45 us against 39, backward 94 against 79, f32 the same.
+// Four need more registers than there are for enough waves: bf16 backward 125 us.
+constexpr int VECTOR = 2;
+// The time axis is split into parts where there are SPLIT steps and the channels make fewer than FILL / 2 workgroups: f16 [333, 37, 100] took 30 us forward and 55 us backward
+// in one part (29 workgroups) and takes 13 and 18 in six.  FILL workgroups are then wanted: 768 or 1024 made bf16 [16384, 4, 256] 10 % slower, 256 made it 15 % slower.
+// SEGMENTS parts at most, because each folds the maps of all before it: 512 made the backward pass of f32 [65536, 1, 128] 40 us instead of 29.
+constexpr int SPLIT = 128, FILL = 512, SEGMENTS = 256;
+constexpr int FOLD = 16;                  // maps of other parts that a wave has on their way at once (4: 4 us of the 21 to 30 us of a long scan's second pass; 32: registers)
 constexpr float LOG2E = 1.44269504088896340736f;
 
-// a = sigmoid(f) and n = 1 - a.  Whichever is below 1/2 is formed without cancellation, the other as 1 minus it, so that a + n = 1 to the last bit of the larger one: what
-// a long memory loses and what it takes in stay in balance whatever the errors of the fast exponential and reciprocal.  f = +-inf gives exactly 1 and 0, a NaN two of them.
+// a = sigmoid(f) and n = 1 - a.  Whichever is below 1/2 is formed without cancellation, the other as 1 minus it: the errors of the fast exponential and reciprocal (1 ulp
+// each) then hit a near 1 only in proportion to n, and what a long memory loses and what it takes in differ by the rounding of a alone.  f = +-inf gives exactly 1 and 0, a NaN two.
 __device__ __forceinline__ void gate(float f, float& a, float& n) {
     const float e = exp2_fast(-fabsf(f) * LOG2E);
     const float lo = e * rcp_fast(1.f + e), hi = 1.f - lo;
     a = f >= 0.f ? hi : lo;
     n = f >= 0.f ? lo : hi;
 }
-__device__ __forceinline__ float sigmoid(float f) { float a, n; gate(f, a, n); return a; }
+// the output gate: nothing is carried on with it, so its own value is enough (o = -inf: 1 / inf = 0)
+__device__ __forceinline__ float sigmoid(float o) { return rcp_fast(1.f + exp2_fast(-o * LOG2E)); }
+// ... and with its derivative s (1 - s) = e / (1 + e)^2, the same for o and -o
+__device__ __forceinline__ void sigmoid_slope(float o, float& s, float& slope) {
+    const float e = exp2_fast(-fabsf(o) * LOG2E), hi = rcp_fast(1.f + e), lo = e * hi;
+    s = o >= 0.f ? hi : lo; slope = lo * hi;
+}
 
 // A run of steps is the map h -> P h + Q.  A reset inside it is P = -0: no product of gates is, products with gates keep it, and it lets nothing of h through (0 times an
 // infinity or a NaN would).
@@ -118,7 +135,7 @@ struct Operand {
 };
 
 // What a step counts for: everything, or - behind a sequence's end, behind the part's - nothing: then a = 1 and n = 0.  Nearly every tile of a wave counts in whole and holds no
-// reset; one vote of the wave decides between that form of the arithmetic and the one with the masks (twice the instructions).
+// reset; one vote of the wave decides between that form of the arithmetic and the one with the masks (twice the instructions: bf16 [32, 4096, 256] backward 82 us with masks alone).
 typedef std::integral_constant<bool, false> Plain;
 typedef std::integral_constant<bool, true> Masked;
 __device__ __forceinline__ bool nowhere(bool x) { return __builtin_amdgcn_ballot_w64(x) == 0; }
@@ -163,8 +180,7 @@ template <int VEC> __device__ __forceinline__ bool plain_steps(const Scan& S, co
     return left == STEPS && (!S.masked || nowhere(resets != 0 || live < STEPS));
 }
 
-// maps of the waves of a workgroup, two tiles' worth in turn: [2][waves][64 VEC] Map forward, [2][waves][3][64 VEC] floats backward (sized by the launch: a static array for WAVES
-// waves would keep workgroups of fewer waves off the CU)
+// maps of the waves of a workgroup, two tiles' worth in turn: [2][waves][64 VEC] Map forward, [2][waves][3][64 VEC] floats backward (sized by the launch)
 APX_DYNAMIC_LDS(Map, scan_lds, 16);
 
 // ------------------------------------------------------------------------------------------------ a split time axis
@@ -251,20 +267,23 @@ __device__ __forceinline__ void enter(const Scan& S, const Channels<VEC>& ch, in
     Map m[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) m[v] = Map{1.f, 0.f};
-    for (int i = i0; i < i1; i += 4) {
-        Map q[4][VEC];
+    auto batch = [&](int i, auto many) {      // that many maps on their way at once: they are what a workgroup waits for first
+        constexpr int N = many;
+        Map q[N][VEC];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < N; ++k) {
             const int at = i + k < i1 ? i + k : i;
             const Map* p = S.maps + (int64_t)(BACK ? S.segments - 1 - at : at) * S.B * S.H + ch.c;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) q[k][v] = p[v];
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < N; ++k)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) if (i + k < i1) m[v] = then(m[v], q[k][v]);
-    }
+    };
+    if (share > 4) for (int i = i0; i < i1; i += FOLD) batch(i, std::integral_constant<int, FOLD>());
+    else if (i0 < i1) batch(i0, std::integral_constant<int, 4>());
 #pragma unroll
     for (int v = 0; v < VEC; ++v) L[w * 64 * VEC + lane * VEC + v] = m[v];
     __syncthreads();
@@ -277,7 +296,8 @@ __device__ __forceinline__ void enter(const Scan& S, const Channels<VEC>& ch, in
 // ------------------------------------------------------------------------------------------------ forward
 // A workgroup walks a part of the time axis of 64 VEC channels in tiles of nw x STEPS steps.  A wave holds its STEPS steps of a tile in registers, the maps of the waves' steps
 // meet in LDS (one barrier a tile, two buffers in turn), each wave then runs its own steps again from the state that enters them: one read of the inputs, no step of the chain
-// longer than STEPS + nw multiply-adds.  Without an output gate the next tile's loads are issued before this one's barrier (with one there are not the registers for it).
+// longer than STEPS + nw multiply-adds.  Without an output gate the next tile's loads are issued before this one's barrier (f32 [400, 1024, 128] 158 -> 131 us); with one there are not
+// the registers for it (175 -> 190 us).
 template <int TYPE, int VEC, bool GATE>
 __global__ __launch_bounds__(64 * WAVES) void gated_scan_fwd_kernel(Scan S) {
     typedef Row<TYPE, VEC> R;
@@ -387,7 +407,8 @@ __global__ __launch_bounds__(64 * WAVES) void gated_scan_fwd_kernel(Scan S) {
 
 // ------------------------------------------------------------------------------------------------ backward
 // The same walk from the end.  A tile begins with a kept state; the waves' maps of h (forward in time) and of c (backward: the same product of gates) meet in LDS together.  A wave
-// then runs its steps forward for the states and backward for the gradients, on registers alone.
+// then runs its steps forward for the states and backward for the gradients, on registers alone.  (f32 without an output gate needs 183 of them, with one 229: 2 waves a SIMD,
+// enough for the memory.  Held to 128 by the launch bounds the compiler spills: 700 us for 305.  The output gate is evaluated twice rather than kept.)
 template <int TYPE, int VEC, bool GATE>
 __global__ __launch_bounds__(64 * WAVES) void gated_scan_bwd_kernel(Scan S) {
     typedef Row<TYPE, VEC> R;
@@ -497,9 +518,9 @@ __global__ __launch_bounds__(64 * WAVES) void gated_scan_bwd_kernel(Scan S) {
                     h[v] = fmaf(a[i][v], p, n[i][v] * x[i][v]);
                     x[i][v] = (p - x[i][v]) * (a[i][v] * n[i][v]);
                     if constexpr (GATE) {
-                        float g, r;
-                        gate(R::get(ro[i], v), g, r);
-                        out[v] = counts(i) ? d[i][v] * h[v] * (g * r) : 0.f;
+                        float g, slope;
+                        sigmoid_slope(R::get(ro[i], v), g, slope);
+                        out[v] = counts(i) ? d[i][v] * h[v] * slope : 0.f;
                         d[i][v] = counts(i) ? d[i][v] * g : 0.f;
                     }
                 }
@@ -596,8 +617,7 @@ Scan scan_of(const apx_gated_scan_args* a) {
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-// How the time axis is split: where the channels alone do not fill the chip, into parts of whole kept stretches (a part costs a second look at f and x, and folds the maps of the
-// parts before it).
+// how the time axis is split: into parts of whole kept stretches
 struct Split { int64_t groups, segment; int segments; };
 Split split(int64_t T, int64_t BH, int vec) {
     Split p;
@@ -625,6 +645,7 @@ template <int TYPE, int VEC, bool GATE> int launch(Scan S, bool back, hipStream_
                     (S.T <= 1 ? 0 : (STEPS - 1) * st->t) + last * (last ? st->b : 0) + 4ll * S.H < ((int64_t)1 << 32), "neighbouring steps or sequences lie too far apart");
     APX_REQUIRE((STEPS - 1) * S.B + last < ((int64_t)1 << 32), "B");
     const dim3 grid((unsigned)p.groups, p.segments), block(64 * waves(S.T < p.segment ? S.T : p.segment));
+    APX_REQUIRE(p.groups * block.x < ((int64_t)1 << 32), "B * H");
     const size_t maps = block.x * VEC * sizeof(Map);      // LDS for one map a thread and channel
     if (p.segments > 1) {
         if (back) hipLaunchKernelGGL((gated_scan_maps_kernel<TYPE, VEC, GATE, true>), grid, block, maps, s, S);
@@ -705,7 +726,7 @@ extern "C" int apx_gated_scan_step(const apx_gated_scan_args* a, float* h, void*
     a = &one;
     if (const int rc = check_common(a)) return rc;
     if (a->B == 0 || a->H == 0) return APX_OK;
-    APX_REQUIRE(h, "h");
+    APX_REQUIRE(h && a->B * a->H < ((int64_t)1 << 31), "h, B * H");
     APX_SCAN_IN(f, f); APX_SCAN_IN(x, x); APX_SCAN_OUT(y, y);
     if (a->o) APX_SCAN_IN(o, o);
     APX_REQUIRE(a->y != a->f && a->y != a->x && a->y != a->o && a->y != (const void*)h, "y must not lie on an input or on h");

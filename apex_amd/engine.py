@@ -230,13 +230,21 @@ def _like(f):
     return torch.empty_like(f, memory_format=torch.contiguous_format)
 
 
+def _output(name, t, f, dev):
+    if t is not None:
+        return _operand(name, t, f, dev, True)
+    t = _like(f)
+    return t, (t.data_ptr(), f.shape[1] * f.shape[2], f.shape[2])
+
+
 def _extra(name, t, shape, dtype, like, dev):
     """t as a dense tensor of that shape and type, and its pointer"""
     if t is None:
         return None, 0
-    if tuple(t.shape) != shape or t.dtype != dtype or t.get_device() != dev:
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
         raise ValueError("%s is %s %s on %s, expected %s %s on %s" % (name, tuple(t.shape), t.dtype, t.device, shape, dtype, like.device))
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t, t.data_ptr()
 
 
@@ -245,16 +253,17 @@ _SHAPE, _DTYPE = operator.attrgetter("shape"), operator.attrgetter("dtype")
 
 
 def _scan_inputs(f, x, o, h0, reset, lens, dim=3):
-    _need_gpu(f, x, o, h0, reset, lens)
+    dev = f.get_device()
+    if dev < 0:
+        _need_gpu(f)
     shape, kind = f.shape, _TYPES.get(f.dtype)
     if len(shape) != dim or kind is None:
         raise ValueError("f is %s %s, expected [%sB, H] in f32, bf16 or f16" % (tuple(shape), f.dtype, "T, " if dim == 3 else ""))
-    dev = f.get_device()
     T, B, H = shape if dim == 3 else (1, *shape)
     f, f3 = _operand("f", f, f, dev); x, x3 = _operand("x", x, f, dev); o, o3 = _operand("o", o, f, dev) if o is not None else (None, _NONE)
-    h0, h0p = _extra("h0", h0, (B, H), torch.float32, f, dev)
-    reset, rp = _extra("reset", reset, (T, B) if dim == 3 else (B,), torch.uint8, f, dev)
-    lens, lp = _extra("lens", lens, (B,), torch.int32, f, dev)
+    h0, h0p = _extra("h0", h0, shape[-2:], torch.float32, f, dev) if h0 is not None else (None, 0)
+    reset, rp = _extra("reset", reset, shape[:-1], torch.uint8, f, dev) if reset is not None else (None, 0)
+    lens, lp = _extra("lens", lens, (B,), torch.int32, f, dev) if lens is not None else (None, 0)
     return (kind, H, T, B, *f3, *x3, *o3, h0p, rp, lp), dev, (f, x, o, h0, reset, lens)      # (the tensors that the numbers point into)
 
 
@@ -276,7 +285,7 @@ def gated_scan(f, x, o=None, h0=None, reset=None, lens=None, keep=False, out=Non
         return _elsewhere(gated_scan, dev, f, x, o, h0, reset, lens, keep, out)
     lib = _lib.load()
     _, H, T, B = head[:4]
-    y, y3 = _operand("out", _like(f) if out is None else out, f, dev, True)
+    y, y3 = _output("out", out, f, dev)
     h_last = torch.empty(B, H, dtype=torch.float32, device=f.device)
     save = torch.empty(lib.apx_gated_scan_save_floats(T, B, H), dtype=torch.float32, device=f.device) if keep else None
     ws, wp, wn = _scan_workspace(lib, T, B, H, f)
@@ -289,7 +298,6 @@ def gated_scan_backward(f, x, dy, save, o=None, h0=None, reset=None, lens=None, 
     """Gradients of gated_scan(f, x, o, h0, reset, lens, keep=True) for dy [T, B, H] and dh_last [B, H] f32 (None: 0): (df, dx, do, dh0), do None without o, dh0 f32 and None
     without h0.  out: (df, dx) or (df, dx, do) to write into - slices of one gradient of the product that made f | x | o, for instance."""
     head, dev, held = _scan_inputs(f, x, o, h0, reset, lens)
-    _need_gpu(dy, save, dh_last)
     if dev >= 0 and dev != torch._C._cuda_getDevice():
         return _elsewhere(gated_scan_backward, dev, f, x, dy, save, o, h0, reset, lens, dh_last, out)
     lib = _lib.load()
@@ -300,12 +308,11 @@ def gated_scan_backward(f, x, dy, save, o=None, h0=None, reset=None, lens=None, 
         raise ValueError("save has %d entries, gated_scan(keep=True) on these inputs makes %d" % (save.numel(), n))
     dh_last, dhp = _extra("dh_last", dh_last, (B, H), torch.float32, f, dev)
     k = 2 if o is None else 3
-    if out is None:
-        out = [_like(f) for _ in range(k)]
-    elif len(out) != k:
+    if out is not None and len(out) != k:
         raise ValueError("out holds %d tensors, expected %d" % (len(out), k))
-    df, df3 = _operand("df", out[0], f, dev, True); dx, dx3 = _operand("dx", out[1], f, dev, True)
-    do, do3 = _operand("do", out[2], f, dev, True) if o is not None else (None, _NONE)
+    out = out or (None, None, None)
+    df, df3 = _output("df", out[0], f, dev); dx, dx3 = _output("dx", out[1], f, dev)
+    do, do3 = _output("do", out[2], f, dev) if o is not None else (None, _NONE)
     dh0 = torch.empty(B, H, dtype=torch.float32, device=f.device) if h0 is not None else None
     ws, wp, wn = _scan_workspace(lib, T, B, H, f)
     a = _lib.GatedScanArgs.from_buffer_copy(_SCAN_ARGS.pack(*head, *_NONE, 0, save.data_ptr(), *dy3, dhp, *df3, *dx3, *do3, dh0.data_ptr() if dh0 is not None else 0, wp, wn))
@@ -317,12 +324,14 @@ def gated_scan_step(f, x, h, o=None, reset=None, out=None):
     """One step of gated_scan for a rollout: f, x, o [B, H], the carried state h [B, H] f32 updated in place (rows whose reset byte, uint8 [B], is non-zero start from zero);
     returns y [B, H]."""
     head, dev, held = _scan_inputs(f, x, o, None, reset, None, 2)
-    _need_gpu(h)
     if dev >= 0 and dev != torch._C._cuda_getDevice():
         return _elsewhere(gated_scan_step, dev, f, x, h, o, reset, out)
     if h.shape != f.shape or h.dtype != torch.float32 or h.get_device() != dev or not h.is_contiguous():
         raise ValueError("h is %s %s on %s, expected a dense %s f32 on %s" % (tuple(h.shape), h.dtype, h.device, tuple(f.shape), f.device))
-    y, y3 = _operand("out", _like(f) if out is None else out, f, dev, True)
+    if out is None:
+        y = _like(f); y3 = (y.data_ptr(), 0, f.shape[1])
+    else:
+        y, y3 = _operand("out", out, f, dev, True)
     a = _lib.GatedScanArgs.from_buffer_copy(_SCAN_ARGS.pack(*head, *y3, 0, 0, *_NONE, 0, *_NONE, *_NONE, *_NONE, 0, 0, 0))
     check(_lib.load().apx_gated_scan_step(C.byref(a), C.c_void_p(h.data_ptr()), _stream()))
     return y

@@ -154,11 +154,13 @@ def test_refusals_of_the_c_entry_points():
     F, Bk = lib.apx_gated_scan_forward, lib.apx_gated_scan_backward
     calls = [scan(F, type=3), scan(F, type=-1), scan(F, T=-1), scan(F, B=-1), scan(F, H=-1), scan(F, f=None), scan(F, x=None), scan(F, y=None), scan(F, h_last=None),
              scan(F, f_t=-8), scan(F, y_b=3), scan(F, y_t=7), scan(F, y_t=0), scan(F, y=one), scan(F, h0=4 * one), scan(F, o=9 * one, o_t=-1), scan(F, T=1 << 58), scan(F, B=1 << 35),
-             scan(F, f_t=1 << 60), scan(F, f_t=1 << 30), scan(F, x_b=1 << 30), scan(Bk, dy_b=1 << 31), scan(Bk, save=None), scan(Bk, dy=None), scan(Bk, df=7 * one), scan(Bk, df=one), scan(Bk, o=9 * one, o_t=8, o_b=4), scan(Bk, dx_b=0),
+             scan(F, f_t=1 << 60), scan(F, f_t=1 << 30), scan(F, x_b=1 << 30), scan(F, T=64, B=1 << 20, H=1 << 12, f_b=1 << 12, x_b=1 << 12, y_b=1 << 12, f_t=1 << 32, x_t=1 << 32, y_t=1 << 32), scan(Bk, dy_b=1 << 31), scan(Bk, save=None), scan(Bk, dy=None), scan(Bk, df=7 * one), scan(Bk, df=one), scan(Bk, o=9 * one, o_t=8, o_b=4), scan(Bk, dx_b=0),
              scan(Bk, dh0=11 * one, dh_last=11 * one)]
     s = _lib.GatedScanArgs(type=0, H=4, B=2, f=one, f_b=4, x=2 * one, x_b=4, y=3 * one, y_b=4)
     calls.append(lib.apx_gated_scan_step(C.byref(s), None, None))
     s.y_b = 2
+    calls.append(lib.apx_gated_scan_step(C.byref(s), 4 * one, None))
+    s.B, s.H, s.f_b, s.x_b, s.y_b = 1 << 20, 1 << 12, 1 << 12, 1 << 12, 1 << 12
     calls.append(lib.apx_gated_scan_step(C.byref(s), 4 * one, None))
     calls += [lib.apx_gated_scan_step(None, 4 * one, None), F(None, None), Bk(None, None), lib.apx_adamw(None, None)]
 
