@@ -309,7 +309,8 @@ int64_t entries_of(int n_tensors, const int64_t* numel) {
     for (int i = 0; i < n_tensors; ++i) k += numel[i] > 0 ? (numel[i] + ENTRY - 1) / ENTRY : 0;
     return k;
 }
-int launches_of(int n_tensors, const int64_t* numel) { return (int)((entries_of(n_tensors, numel) + TABLE - 1) / TABLE); }
+// (one even where there is nothing: it counts the step)
+int launches_of(int n_tensors, const int64_t* numel) { const int64_t k = entries_of(n_tensors, numel); return k ? (int)((k + TABLE - 1) / TABLE) : 1; }
 
 }  // namespace
 

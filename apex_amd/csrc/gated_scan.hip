@@ -596,12 +596,13 @@ bool reaches(int64_t T, int64_t B, int H, int64_t st, int64_t sb) {
         APX_REQUIRE(need == 0 || (a->workspace && ((uintptr_t)a->workspace & 15) == 0 && a->workspace_bytes >= need), "workspace");                \
     } while (0)
 
+bool sizes_fit(int64_t T, int64_t B, int H) {
+    return T >= 0 && B >= 0 && H >= 0 && T < ((int64_t)1 << 40) && (__int128)B * H < ((__int128)1 << 36) && (__int128)B * H * (T + 1) < ((__int128)1 << 59);
+}
 int check_common(const apx_gated_scan_args* a) {
     APX_REQUIRE(a, "args");
     APX_REQUIRE(a->type == APX_F32 || a->type == APX_BF16 || a->type == APX_F16, "type");
-    APX_REQUIRE(a->T >= 0 && a->B >= 0 && a->H >= 0 && a->T < ((int64_t)1 << 40), "T, B, H");
-    APX_REQUIRE((__int128)a->B * a->H < ((__int128)1 << 36), "B * H");
-    APX_REQUIRE((__int128)a->B * a->H * (a->T + 1) < ((__int128)1 << 59), "T * B * H");
+    APX_REQUIRE(sizes_fit(a->T, a->B, a->H), "T, B, H");
     return APX_OK;
 }
 Scan scan_of(const apx_gated_scan_args* a) {
@@ -677,10 +678,10 @@ int run(int type, Scan& S, bool back, void* workspace, hipStream_t s) {
     } while (0)
 
 extern "C" size_t apx_gated_scan_save_floats(int64_t T, int64_t B, int H) {
-    return T > 0 && B > 0 && H > 0 ? (size_t)((T + KEEP - 1) / KEEP) * (size_t)B * (size_t)H : 0;
+    return T > 0 && B > 0 && H > 0 && sizes_fit(T, B, H) ? (size_t)((T + KEEP - 1) / KEEP) * (size_t)B * (size_t)H : 0;
 }
 extern "C" size_t apx_gated_scan_workspace_bytes(int64_t T, int64_t B, int H) {
-    if (T <= 0 || B <= 0 || H <= 0) return 0;
+    if (T <= 0 || B <= 0 || H <= 0 || !sizes_fit(T, B, H)) return 0;
     const Split p = split(T, B * H, H % VECTOR == 0 ? VECTOR : 1);
     return p.segments > 1 ? (size_t)p.segments * B * H * sizeof(Map) : 0;
 }

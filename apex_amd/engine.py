@@ -421,6 +421,8 @@ class AdamW:
         """(m, v) flat [elements], in f32 or - 8-bit moments - as the values they stand for in bf16; views() cuts them into the tensors' shapes."""
         if self.state_bits == 32:
             return self.m, self.v
+        if self._index >= 0 and self._index != torch._C._cuda_getDevice():
+            return _elsewhere(self.moments, self._index)
         m, v = (torch.empty(self.elements, dtype=torch.bfloat16, device=self.device) for _ in range(2))
         check(_lib.load().apx_adamw_moments(_p(self.m), _p(self.v), _p(self.m_scale), _p(self.v_scale), self.elements, _p(m), _p(v), _stream()))
         return m, v

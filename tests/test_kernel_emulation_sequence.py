@@ -88,6 +88,17 @@ def test_emulated_adamw_special_blocks(dev):  # noqa: F811
     assert torch.isnan(m[:256]).all() and not m[256:].any() and not v[256:].any() and torch.isnan(p[0][3]) and torch.isfinite(p[0][4:]).all() and torch.equal(p[1], torch.ones(5))
 
 
+def test_emulated_adamw_of_nothing(dev):  # noqa: F811
+    """empty tensors alone: the step counts, the norm is 0"""
+    from apex_amd import engine
+    for bits in (8, 32):
+        o = engine.AdamW([torch.zeros(0), torch.zeros(3, 0)], max_norm=1.0, state_bits=bits)
+        assert o._ws.numel() >= 64 + 8      # (room for the one partial sum of the launch that counts)
+        o.norm.fill_(5.0)
+        o.step([torch.zeros(0), torch.zeros(3, 0)])
+        assert int(o.t) == 1 and float(o.norm) == 0.0 and o.moments()[0].numel() == 0
+
+
 def test_emulated_adamw_rounding_keeps_the_mean(dev):  # noqa: F811
     """4096 elements that all hold the same moments: m = 0.1 g, v = 0.001 g^2 in the first step, rounded up or down to neighbours an eighth of a power of two apart.  The mean of n
     independent roundings is off by at most (step / 2) / sqrt(n) in the standard deviation: five of them here."""
