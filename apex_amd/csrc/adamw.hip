@@ -333,6 +333,7 @@ extern "C" int apx_adamw(const apx_adamw_args* a, void* stream) {
     APX_REQUIRE(a && a->n_tensors >= 0, "args");
     if (a->n_tensors == 0) return APX_OK;
     APX_REQUIRE(a->params && a->grads && a->numel && a->t, "null pointer");
+    APX_REQUIRE((((uintptr_t)a->t | (uintptr_t)a->norm_out) & 7) == 0, "t, norm_out: 8-byte alignment");
     APX_REQUIRE(a->grad_type == APX_F32 || a->grad_type == APX_BF16 || a->grad_type == APX_F16, "grad_type");
     APX_REQUIRE(a->state_bits == 32 || a->state_bits == 8, "state_bits");
     APX_REQUIRE(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1, "beta1, beta2");
@@ -341,6 +342,7 @@ extern "C" int apx_adamw(const apx_adamw_args* a, void* stream) {
     for (int i = 0; i < a->n_tensors; ++i) {
         APX_REQUIRE(a->numel[i] >= 0 && a->numel[i] < ((int64_t)1 << 39), "numel");
         APX_REQUIRE(a->numel[i] == 0 || (a->params[i] && a->grads[i]), "null tensor");
+        APX_REQUIRE(a->numel[i] == 0 || (((uintptr_t)a->params[i] & 3) == 0 && ((uintptr_t)a->grads[i] & (a->grad_type == APX_F32 ? 3 : 1)) == 0), "tensor alignment");
         APX_REQUIRE(!a->weight_decay || std::isfinite(a->weight_decay[i]), "weight_decay");
         total += a->numel[i];
     }
@@ -402,7 +404,7 @@ extern "C" int apx_adamw_moments(const void* m, const void* v, const float* m_sc
     APX_REQUIRE(elements >= 0 && elements % BLOCK == 0, "elements: whole blocks of 256");
     if (elements == 0) return APX_OK;
     APX_REQUIRE(m && v && m_scale && v_scale && m_out && v_out, "null pointer");
-    APX_REQUIRE((((uintptr_t)m | (uintptr_t)v) & 7) == 0 && (((uintptr_t)m_out | (uintptr_t)v_out) & 15) == 0, "alignment");
+    APX_REQUIRE((((uintptr_t)m_scale | (uintptr_t)v_scale) & 3) == 0 && (((uintptr_t)m | (uintptr_t)v) & 7) == 0 && (((uintptr_t)m_out | (uintptr_t)v_out) & 15) == 0, "alignment");
     const int64_t want = (elements + 2047) / 2048;
     hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)(want < GRID ? want : GRID)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)m, (const uint8_t*)v, m_scale, v_scale,
                        elements, (uint16_t*)m_out, (uint16_t*)v_out);

@@ -588,8 +588,10 @@ bool reaches(int64_t T, int64_t B, int H, int64_t st, int64_t sb) {
     const __int128 last = (__int128)(T > 0 ? T - 1 : 0) * st + (__int128)(B > 0 ? B - 1 : 0) * sb + H;
     return st >= 0 && sb >= 0 && last < ((__int128)1 << 60);
 }
-#define APX_SCAN_IN(p, s) APX_REQUIRE(a->p && reaches(a->T, a->B, a->H, a->s##_t, a->s##_b), "input pointer / strides")
-#define APX_SCAN_OUT(p, s) APX_REQUIRE(a->p && reaches(a->T, a->B, a->H, a->s##_t, a->s##_b) && apart(a->T, a->B, a->H, a->s##_t, a->s##_b), "output pointer / strides")
+bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+size_t size_of(int type) { return type == APX_F32 ? 4 : 2; }
+#define APX_SCAN_IN(p, s) APX_REQUIRE(a->p && aligned(a->p, size_of(a->type)) && reaches(a->T, a->B, a->H, a->s##_t, a->s##_b), "input pointer / strides")
+#define APX_SCAN_OUT(p, s) APX_REQUIRE(a->p && aligned(a->p, size_of(a->type)) && reaches(a->T, a->B, a->H, a->s##_t, a->s##_b) && apart(a->T, a->B, a->H, a->s##_t, a->s##_b), "output pointer / strides")
 #define APX_SCAN_WORKSPACE()                                                                                              \
     do {                                                                                                                  \
         const size_t need = apx_gated_scan_workspace_bytes(a->T, a->B, a->H);                                             \
@@ -603,13 +605,15 @@ int check_common(const apx_gated_scan_args* a) {
     APX_REQUIRE(a, "args");
     APX_REQUIRE(a->type == APX_F32 || a->type == APX_BF16 || a->type == APX_F16, "type");
     APX_REQUIRE(sizes_fit(a->T, a->B, a->H), "T, B, H");
+    for (const void* p : {(const void*)a->h0, (const void*)a->lens, (const void*)a->h_last, (const void*)a->save, (const void*)a->dh_last, (const void*)a->dh0})
+        APX_REQUIRE(aligned(p, 4), "4-byte alignment");
     return APX_OK;
 }
 Scan scan_of(const apx_gated_scan_args* a) {
     Scan S = {};
     S.T = a->T; S.B = a->B; S.H = a->H;
     S.f = a->f; S.x = a->x; S.o = a->o; S.dy = a->dy; S.y = a->y; S.df = a->df; S.dx = a->dx; S.do_ = a->do_;
-    const int64_t e = a->type == APX_F32 ? 4 : 2;
+    const int64_t e = size_of(a->type);
     S.sf = {a->f_t * e, a->f_b * e}; S.sx = {a->x_t * e, a->x_b * e}; S.so = {a->o_t * e, a->o_b * e}; S.sy = {a->y_t * e, a->y_b * e};
     S.sdy = {a->dy_t * e, a->dy_b * e}; S.sdf = {a->df_t * e, a->df_b * e}; S.sdx = {a->dx_t * e, a->dx_b * e}; S.sdo = {a->do_t * e, a->do_b * e};
     S.h0 = a->h0; S.dh_last = a->dh_last; S.h_last = a->h_last; S.save = a->save; S.dh0 = a->dh0;
@@ -640,11 +644,11 @@ template <int TYPE, int VEC, bool GATE> int launch(Scan S, bool back, hipStream_
     S.segment = p.segment; S.segments = p.segments;
     S.masked = S.reset || S.lens;
     // what a wave touches in a tile - STEPS steps of the sequences that its 64 VEC channels belong to - lies within 4 GB; `last`: how many sequences behind its first one
-    const int64_t n = 64 * VEC, more = S.H % n == 0 ? 0 : n % S.H == 0 ? n / S.H - 1 : n / S.H + 1, last = S.B - 1 < more ? S.B - 1 : more;
+    const int64_t steps = (S.T < STEPS ? S.T : STEPS) - 1, n = 64 * VEC, more = S.H % n == 0 ? 0 : n % S.H == 0 ? n / S.H - 1 : n / S.H + 1, last = S.B - 1 < more ? S.B - 1 : more;
     for (const Strides* st : {&S.sf, &S.sx, &S.so, &S.sy, &S.sdy, &S.sdf, &S.sdx, &S.sdo})
         APX_REQUIRE((S.T <= 1 || st->t < ((int64_t)1 << 32)) && (last == 0 || st->b < ((int64_t)1 << 32)) &&
-                    (S.T <= 1 ? 0 : (STEPS - 1) * st->t) + last * (last ? st->b : 0) + 4ll * S.H < ((int64_t)1 << 32), "neighbouring steps or sequences lie too far apart");
-    APX_REQUIRE((STEPS - 1) * S.B + last < ((int64_t)1 << 32), "B");
+                    (S.T <= 1 ? 0 : steps * st->t) + last * (last ? st->b : 0) + 4ll * S.H < ((int64_t)1 << 32), "neighbouring steps or sequences lie too far apart");
+    APX_REQUIRE((S.T <= 1 ? 0 : steps * S.B) + last < ((int64_t)1 << 32), "B");
     const dim3 grid((unsigned)p.groups, p.segments), block(64 * waves(S.T < p.segment ? S.T : p.segment));
     APX_REQUIRE(p.groups * block.x < ((int64_t)1 << 32), "B * H");
     const size_t maps = block.x * VEC * sizeof(Map);      // LDS for one map a thread and channel
@@ -727,7 +731,7 @@ extern "C" int apx_gated_scan_step(const apx_gated_scan_args* a, float* h, void*
     a = &one;
     if (const int rc = check_common(a)) return rc;
     if (a->B == 0 || a->H == 0) return APX_OK;
-    APX_REQUIRE(h && a->B * a->H < ((int64_t)1 << 31), "h, B * H");
+    APX_REQUIRE(h && aligned(h, 4) && a->B * a->H < ((int64_t)1 << 31), "h, B * H");
     APX_SCAN_IN(f, f); APX_SCAN_IN(x, x); APX_SCAN_OUT(y, y);
     if (a->o) APX_SCAN_IN(o, o);
     APX_REQUIRE(a->y != a->f && a->y != a->x && a->y != a->o && a->y != (const void*)h, "y must not lie on an input or on h");

@@ -135,7 +135,10 @@ int apx_lstm_backward(const float* params, float* grads, int D, int H, int L, in
  * product need no copy.  Inputs may overlap or repeat (stride 0); outputs must not overlap each other or an input, nor themselves.  h0, h_last, save, dh_last, dh0: f32,
  * dense [B, H].  reset: u8, dense [T, B].  lens: i32 [B], below 0 taken as 0 and above T as T.  States, gates and sums are f32 whatever the type; each output is rounded once.
  * workspace: apx_gated_scan_workspace_bytes bytes (0 for most shapes: then it may be NULL), 16-byte aligned, not shared by calls that may run at the same time.
- * Results do not depend on anything but the inputs and shapes (no atomics).  T = 0, B = 0 and H = 0 are allowed. all pointers [dev] */
+ * Every pointer is aligned to its own type.  Eight neighbouring steps of the sequences that share 128 channels (64 where H is odd) lie within 4 GB in every operand (T = 1: those
+ * sequences' rows alone); calls beyond that are refused.
+ * Results do not depend on anything but the inputs and shapes (no atomics).  A NaN stays in its channel until a reset, and so does an infinity, which may become a NaN on the
+ * way (the steps between are joined by the products of their gates, and 0 times an infinity is one).  T = 0, B = 0 and H = 0 are allowed. all pointers [dev] */
 #define APX_F32 0
 #define APX_BF16 1
 #define APX_F16 2
@@ -282,8 +285,8 @@ int apx_clip_adam(float* param, float* m, float* v, float* grad, int64_t n, floa
  * with the probability that keeps their mean (rounded to nearest, a v that moves by 1 - beta2 of itself a step would never leave its code); a v > 0 below the range takes the
  * smallest code, not 0.  A block that holds an infinity, a NaN or a value of 2^127 and more reads back as NaN.  The update itself uses the moments before this rounding.
  * t: i64 [dev], the steps taken so far, counted up here (so that a captured step counts when it is replayed).
- * workspace: apx_adamw_workspace_bytes bytes, 16-byte aligned.  params / grads may have any alignment
- * their type allows, m / v and their scales are 4-byte aligned.  Sums run in a fixed order (no atomics).
+ * workspace: apx_adamw_workspace_bytes bytes, 16-byte aligned, not shared by calls that may run at the same time.  params / grads may have any alignment their type allows,
+ * m / v and their scales are 4-byte, t and norm_out 8-byte aligned.  Sums run in a fixed order (no atomics).
  * apx_adamw_moments: 8-bit moments as the values they stand for, in bf16 (which holds them exactly); codes 8-byte, outputs 16-byte aligned. */
 typedef struct apx_adamw_args {
     int n_tensors, grad_type, state_bits;

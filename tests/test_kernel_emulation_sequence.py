@@ -197,6 +197,51 @@ def test_refusals_of_the_c_entry_points():
     assert lib.apx_adamw_state_elements(3, (C.c_int64 * 3)(1, 0, 257)) == 768
 
 
+def test_refusals_of_misaligned_pointers():
+    """a pointer that is not aligned to its own type is refused at every C entry"""
+    from apex_amd import _lib
+    lib = _lib.load()
+    p = lambda k: 64 * k  # noqa: E731
+    for kind, half in ((0, 2), (1, 1), (2, 1)):
+        good = dict(type=kind, H=4, T=3, B=2, f=p(1), f_t=8, f_b=4, x=p(2), x_t=8, x_b=4, y=p(3), y_t=8, y_b=4, h_last=p(4), dy=p(5), dy_t=8, dy_b=4, df=p(6), df_t=8, df_b=4,
+                    dx=p(7), dx_t=8, dx_b=4, save=p(8), o=p(9), o_t=8, o_b=4, do_=p(10), do_t=8, do_b=4, h0=p(11), dh0=p(12), dh_last=p(13), lens=p(14))
+        call = lambda fn, k, by: fn(C.byref(_lib.GatedScanArgs(**{**good, k: good[k] + by})), None)  # noqa: E731
+        assert [call(lib.apx_gated_scan_forward, k, half) for k in "fxoy"] == [-1] * 4
+        assert [call(lib.apx_gated_scan_backward, k, half) for k in ("f", "x", "o", "dy", "df", "dx", "do_")] == [-1] * 7
+        assert [call(lib.apx_gated_scan_forward, k, 2) for k in ("h0", "h_last", "lens", "save")] == [-1] * 4
+        assert [call(lib.apx_gated_scan_backward, k, 2) for k in ("h0", "dh0", "dh_last", "lens", "save")] == [-1] * 5
+        step = _lib.GatedScanArgs(**{**good, "h0": 0, "lens": 0})
+        assert lib.apx_gated_scan_step(C.byref(step), p(15) + 2, None) == -1
+
+    def adam(kind, at, gat, **change):
+        ptr, grad, num = (C.c_void_p * 1)(at), (C.c_void_p * 1)(gat), (C.c_int64 * 1)(5)
+        a = _lib.AdamwArgs(n_tensors=1, grad_type=kind, state_bits=32, params=C.addressof(ptr), grads=C.addressof(grad), numel=C.addressof(num), m=p(2), v=p(3), t=p(4), lr=1e-3, beta1=0.9,
+                           beta2=0.999, eps=1e-8, grad_scale=1.0, max_norm=1.0, workspace=p(5), workspace_bytes=1 << 20, norm_out=p(6))
+        for k, v in change.items():
+            setattr(a, k, v)
+        return lib.apx_adamw(C.byref(a), None)
+    assert [adam(0, p(1) + 2, p(7)), adam(0, p(1), p(7) + 2), adam(1, p(1), p(7) + 1), adam(2, p(1), p(7) + 1), adam(0, p(1), p(7), t=p(4) + 4), adam(0, p(1), p(7), norm_out=p(6) + 4),
+            adam(0, p(1), p(7), m=p(2) + 2)] == [-1] * 7
+    assert [lib.apx_adamw_moments(*a, None) for a in ((p(1) + 4, p(2), p(3), p(4), 256, p(5), p(6)), (p(1), p(2), p(3) + 2, p(4), 256, p(5), p(6)), (p(1), p(2), p(3), p(4), 256, p(5) + 8, p(6)))] == [-1] * 3
+
+
+def test_emulated_scan_of_two_far_steps(dev):  # noqa: F811
+    """what has to lie within 4 GB are a call's own steps: two of them 2 GB apart are served, with three of them (4 GB) refused"""
+    from apex_amd import _lib
+    lib = _lib.load()
+    a = dict(type=0, H=4, B=1, f=64, f_b=4, x=128, x_t=4, x_b=4, y=192, y_t=4, y_b=4, h_last=256)
+    assert lib.apx_gated_scan_forward(C.byref(_lib.GatedScanArgs(T=3, f_t=1 << 29, **a)), None) == -1 and b"too far apart" in lib.apx_last_error()
+    import mmap
+    far = mmap.mmap(-1, (1 << 31) + 4096)      # (touched at its two ends alone)
+    f = torch.frombuffer(far, dtype=torch.float32, count=(1 << 29) + 4).as_strided((2, 1, 4), (1 << 29, 4, 1))
+    f.copy_(torch.randn(2, 1, 4))
+    from apex_amd import engine
+    x = torch.randn(2, 1, 4)
+    y, h = engine.gated_scan(f, x)
+    y2, h2 = engine.gated_scan(f.contiguous(), x)
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+
+
 def test_wrappers_need_device_tensors():
     from apex_amd import _lib, engine
     f = torch.zeros(4, 2, 3)
