@@ -129,9 +129,9 @@ SIGNATURES = {
                                 C.c_int, c_ptr, c_ptr]),
     "apx_gated_scan_save_floats": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int]),
     "apx_gated_scan_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int]),
-    "apx_gated_scan_forward": (C.c_int, [C.POINTER(GatedScanArgs), c_ptr]),
-    "apx_gated_scan_backward": (C.c_int, [C.POINTER(GatedScanArgs), c_ptr]),
-    "apx_gated_scan_step": (C.c_int, [C.POINTER(GatedScanArgs), c_ptr, c_ptr]),
+    "apx_gated_scan_forward": (C.c_int, [c_ptr, c_ptr]),      # (the struct: by reference, or its bytes as they are)
+    "apx_gated_scan_backward": (C.c_int, [c_ptr, c_ptr]),
+    "apx_gated_scan_step": (C.c_int, [c_ptr, c_ptr, c_ptr]),
     "apx_adamw_state_elements": (C.c_int64, [C.c_int, c_ptr]),
     "apx_adamw_workspace_bytes": (C.c_size_t, [C.c_int, c_ptr]),
     "apx_adamw": (C.c_int, [C.POINTER(AdamwArgs), c_ptr]),

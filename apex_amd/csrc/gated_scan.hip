@@ -561,19 +561,20 @@ __global__ __launch_bounds__(64 * WAVES) void gated_scan_bwd_kernel(Scan S) {
 }
 
 // ------------------------------------------------------------------------------------------------ one step
+struct OneStep { const void *f, *x, *o; void* y; int64_t fb, xb, ob, yb; const uint8_t* reset; unsigned channels, H; };      // rows so many bytes apart
 template <int TYPE>
-__global__ __launch_bounds__(256) void gated_scan_step_kernel(Scan S, float* __restrict__ h) {
+__global__ __launch_bounds__(256) void gated_scan_step_kernel(OneStep S, float* __restrict__ h) {
     typedef Elem<TYPE> E; typedef typename E::raw raw;
-    const int64_t c = blockIdx.x * (int64_t)256 + threadIdx.x;
-    if (c >= S.B * S.H) return;
-    const int64_t b = c / S.H; const int j = (int)(c - b * S.H);
-    auto at = [&](const void* p, const Strides& st) { return *(const raw*)((const char*)p + b * st.b + j * sizeof(raw)); };
+    const unsigned c = blockIdx.x * 256u + threadIdx.x;
+    if (c >= S.channels) return;
+    const unsigned b = c / S.H, j = c - b * S.H;
+    auto at = [&](const void* p, int64_t row) { return *(const raw*)((const char*)p + b * row + j * sizeof(raw)); };
     float a, n;
-    gate(E::get(at(S.f, S.sf)), a, n);
-    const float v = n * E::get(at(S.x, S.sx));
+    gate(E::get(at(S.f, S.fb)), a, n);
+    const float v = n * E::get(at(S.x, S.xb));
     const float s = S.reset && S.reset[b] ? v : fmaf(a, h[c], v);
     h[c] = s;
-    *(raw*)((char*)S.y + b * S.sy.b + j * sizeof(raw)) = E::put(S.o ? s * sigmoid(E::get(at(S.o, S.so))) : s);
+    *(raw*)((char*)S.y + b * S.yb + j * sizeof(raw)) = E::put(S.o ? s * sigmoid(E::get(at(S.o, S.ob))) : s);
 }
 
 // entries (t, b, j) of an output do not fall on each other: either whole steps follow one another or whole sequences do
@@ -735,7 +736,8 @@ extern "C" int apx_gated_scan_step(const apx_gated_scan_args* a, float* h, void*
     APX_SCAN_IN(f, f); APX_SCAN_IN(x, x); APX_SCAN_OUT(y, y);
     if (a->o) APX_SCAN_IN(o, o);
     APX_REQUIRE(a->y != a->f && a->y != a->x && a->y != a->o && a->y != (const void*)h, "y must not lie on an input or on h");
-    const Scan S = scan_of(a);
+    const int64_t e = size_of(a->type);
+    const OneStep S = {a->f, a->x, a->o, a->y, a->f_b * e, a->x_b * e, a->o_b * e, a->y_b * e, a->reset, (unsigned)(a->B * a->H), (unsigned)a->H};
     APX_BY_TYPE(a->type, gated_scan_step_kernel, apx_cdiv(a->B * a->H, 256), 256, (hipStream_t)stream, S, h);
     return APX_OK;
 }

@@ -205,7 +205,8 @@ class Lstm:
 
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # APX_F32, APX_BF16, APX_F16
-_SCAN_ARGS = struct.Struct("2i35q")      # apx_gated_scan_args: packed in one go (field by field it was 10 us a call, three times a step's kernel)
+# apx_gated_scan_args, packed in one go (field by field it was 10 us a call, three times a step's kernel); a step fills the first fields
+_SCAN_ARGS, _STEP_ARGS = struct.Struct("2i35q"), struct.Struct("2i17q144x")
 
 
 def _elsewhere(fn, dev, *a, **k):
@@ -227,7 +228,7 @@ def _operand(name, t, like, dev, out=False):
 
 
 def _like(f):
-    return torch.empty_like(f, memory_format=torch.contiguous_format)
+    return torch.empty_like(f) if f.is_contiguous() else torch.empty_like(f, memory_format=torch.contiguous_format)
 
 
 def _output(name, t, f, dev):
@@ -252,14 +253,14 @@ _NONE = (0, 0, 0)
 _SHAPE, _DTYPE = operator.attrgetter("shape"), operator.attrgetter("dtype")
 
 
-def _scan_inputs(f, x, o, h0, reset, lens, dim=3):
+def _scan_inputs(f, x, o, h0, reset, lens):
     dev = f.get_device()
     if dev < 0:
         _need_gpu(f)
     shape, kind = f.shape, _TYPES.get(f.dtype)
-    if len(shape) != dim or kind is None:
-        raise ValueError("f is %s %s, expected [%sB, H] in f32, bf16 or f16" % (tuple(shape), f.dtype, "T, " if dim == 3 else ""))
-    T, B, H = shape if dim == 3 else (1, *shape)
+    if len(shape) != 3 or kind is None:
+        raise ValueError("f is %s %s, expected [T, B, H] in f32, bf16 or f16" % (tuple(shape), f.dtype))
+    T, B, H = shape
     f, f3 = _operand("f", f, f, dev); x, x3 = _operand("x", x, f, dev); o, o3 = _operand("o", o, f, dev) if o is not None else (None, _NONE)
     h0, h0p = _extra("h0", h0, shape[-2:], torch.float32, f, dev) if h0 is not None else (None, 0)
     reset, rp = _extra("reset", reset, shape[:-1], torch.uint8, f, dev) if reset is not None else (None, 0)
@@ -289,8 +290,8 @@ def gated_scan(f, x, o=None, h0=None, reset=None, lens=None, keep=False, out=Non
     h_last = torch.empty(B, H, dtype=torch.float32, device=f.device)
     save = torch.empty(lib.apx_gated_scan_save_floats(T, B, H), dtype=torch.float32, device=f.device) if keep else None
     ws, wp, wn = _scan_workspace(lib, T, B, H, f)
-    a = _lib.GatedScanArgs.from_buffer_copy(_SCAN_ARGS.pack(*head, *y3, h_last.data_ptr(), save.data_ptr() if keep else 0, *_NONE, 0, *_NONE, *_NONE, *_NONE, 0, wp, wn))
-    check(lib.apx_gated_scan_forward(C.byref(a), _stream()))
+    a = _SCAN_ARGS.pack(*head, *y3, h_last.data_ptr(), save.data_ptr() if keep else 0, *_NONE, 0, *_NONE, *_NONE, *_NONE, 0, wp, wn)
+    check(lib.apx_gated_scan_forward(a, _stream()))
     return (y, h_last, save) if keep else (y, h_last)
 
 
@@ -315,25 +316,35 @@ def gated_scan_backward(f, x, dy, save, o=None, h0=None, reset=None, lens=None, 
     do, do3 = _output("do", out[2], f, dev) if o is not None else (None, _NONE)
     dh0 = torch.empty(B, H, dtype=torch.float32, device=f.device) if h0 is not None else None
     ws, wp, wn = _scan_workspace(lib, T, B, H, f)
-    a = _lib.GatedScanArgs.from_buffer_copy(_SCAN_ARGS.pack(*head, *_NONE, 0, save.data_ptr(), *dy3, dhp, *df3, *dx3, *do3, dh0.data_ptr() if dh0 is not None else 0, wp, wn))
-    check(lib.apx_gated_scan_backward(C.byref(a), _stream()))
+    a = _SCAN_ARGS.pack(*head, *_NONE, 0, save.data_ptr(), *dy3, dhp, *df3, *dx3, *do3, dh0.data_ptr() if dh0 is not None else 0, wp, wn)
+    check(lib.apx_gated_scan_backward(a, _stream()))
     return df, dx, do, dh0
 
 
 def gated_scan_step(f, x, h, o=None, reset=None, out=None):
     """One step of gated_scan for a rollout: f, x, o [B, H], the carried state h [B, H] f32 updated in place (rows whose reset byte, uint8 [B], is non-zero start from zero);
     returns y [B, H]."""
-    head, dev, held = _scan_inputs(f, x, o, None, reset, None, 2)
+    dev, shape, dtype = f.get_device(), f.shape, f.dtype
+    if dev < 0:
+        _need_gpu(f)
+    kind = _TYPES.get(dtype)
+    if len(shape) != 2 or kind is None:
+        raise ValueError("f is %s %s, expected [B, H] in f32, bf16 or f16" % (tuple(shape), dtype))
     if dev >= 0 and dev != torch._C._cuda_getDevice():
         return _elsewhere(gated_scan_step, dev, f, x, h, o, reset, out)
-    if h.shape != f.shape or h.dtype != torch.float32 or h.get_device() != dev or not h.is_contiguous():
-        raise ValueError("h is %s %s on %s, expected a dense %s f32 on %s" % (tuple(h.shape), h.dtype, h.device, tuple(f.shape), f.device))
+    B, H = shape
+    f, (fp, _, fb) = _operand("f", f, f, dev)
+    x, (xp, _, xb) = _operand("x", x, f, dev)
+    o, (op, _, ob) = _operand("o", o, f, dev) if o is not None else (None, _NONE)
+    reset, rp = _extra("reset", reset, shape[:1], torch.uint8, f, dev) if reset is not None else (None, 0)
+    if h.shape != shape or h.dtype is not torch.float32 or h.get_device() != dev or not h.is_contiguous():
+        raise ValueError("h is %s %s on %s, expected a dense %s f32 on %s" % (tuple(h.shape), h.dtype, h.device, tuple(shape), f.device))
     if out is None:
-        y = _like(f); y3 = (y.data_ptr(), 0, f.shape[1])
+        y = _like(f); yp, yb = y.data_ptr(), H
     else:
-        y, y3 = _operand("out", out, f, dev, True)
-    a = _lib.GatedScanArgs.from_buffer_copy(_SCAN_ARGS.pack(*head, *y3, 0, 0, *_NONE, 0, *_NONE, *_NONE, *_NONE, 0, 0, 0))
-    check(_lib.load().apx_gated_scan_step(C.byref(a), C.c_void_p(h.data_ptr()), _stream()))
+        y, (yp, _, yb) = _operand("out", out, f, dev, True)
+    a = _STEP_ARGS.pack(kind, H, 1, B, fp, 0, fb, xp, 0, xb, op, 0, ob, 0, rp, 0, yp, 0, yb)
+    check(_lib.load().apx_gated_scan_step(a, h.data_ptr(), _stream()))
     return y
 
 
@@ -407,9 +418,10 @@ class AdamW:
             raise ValueError("a tensor of params has moved since this optimiser was made: it works on the memory that it was given")
         if index >= 0 and index != torch._C._cuda_getDevice():
             return _elsewhere(self.step, index, grads, grad_scale, lr)
-        gs = array.array("Q", map(torch.Tensor.data_ptr, grads))
+        gs = list(map(torch.Tensor.data_ptr, grads))
         if not self._taken.isdisjoint(gs):
             raise ValueError("a gradient lies on a tensor of params")
+        gs = array.array("Q", gs)
         if self.max_norm is not None and not self.max_norm > 0:
             raise ValueError("max_norm is %r, expected a positive number or None" % (self.max_norm,))
         a = self._args
