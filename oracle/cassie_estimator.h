@@ -1,7 +1,7 @@
 // CPU ORACLE (test infrastructure only — see oracle/__init__.py): fp64 restatement of the reference's state estimator,
 // `state_output_step` of libcassiemujoco.so (interface: cassie/cassiemujoco/include/StateOutput.h:33-36; consumed by
 // CassieEnv.get_full_state, cassie/cassie.py:817-850).  The routine exists only as machine code; it was decoded from the unstripped
-// binary (disassembly + direct calls of its internal routines + dumps of its 0x1070-byte state object, tools/refprobe/decode_estimator/)
+// binary (disassembly + direct calls of its internal routines + dumps of its 0x1070-byte state object)
 // and is PINNED: golden G11 is the binary's own output on a 3000-substep sensor stream, reproduced here to < 1e-7 on every filtered
 // output incl. start-up (tests/test_oracle_env.py::test_g11_state_estimator_restated).
 //
