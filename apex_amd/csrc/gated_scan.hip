@@ -475,8 +475,11 @@ __global__ __launch_bounds__(64 * WAVES) void gated_scan_bwd_kernel(Scan S) {
                     d[i][v] = y;
                     const float b = n[i][v] * x[i][v];
                     Q = reset ? b : fmaf(a[i][v], Q, b);
-                    P = reset ? -0.f : P * a[i][v];
+                    P *= a[i][v];
                 }
+                // A reset anywhere in the steps cuts both maps.  Of h, that lies in the order of the steps: a gate behind it that is a NaN is one in Q too.  Of c, a NaN behind it must
+                // not come through: the product of gates is not asked.
+                if (masked && (resets & ((1u << live) - 1u))) P = -0.f;
 #pragma unroll
                 for (int i = STEPS - 1; i >= 0; --i) {
                     float g = d[i][v];

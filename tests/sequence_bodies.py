@@ -208,3 +208,51 @@ def check_adamw(dev, shapes, bits=32, grad="f32", clip=None, steps=3, seed=0, wd
     for v, p in zip(opt.views(opt.moments()[0]), ps):
         assert v.shape == p.shape
     return opt, ps
+
+
+# ------------------------------------------------------------------------------------------------ what is not finite at steps that count
+def check_not_finite(dev, T, B, H, t="f32", gate=False, lens=False, infinite=False, seed=0, at=None):
+    """NaN (infinite: and infinities) in f, x, o and dy at steps that count, resets before and behind them: outputs are not finite exactly where the formulas' are, and right
+    everywhere else.  An infinity may become a NaN between two resets (the steps are joined by products of gates), a NaN stays one.  at: the one sequence's (reset, step of a NaN gate)
+    instead of places by chance.
+    Tolerances are those of check_scan: M and L of the finite inputs; G with |dy|, without output gates and with every gate that is not a number open, which is no smaller than any
+    finite |g|."""
+    from apex_amd import engine
+    d, dy, dh = make(T, B, H, t, gate, True, lens, True, dev, seed)
+    r = np.random.RandomState(seed + 1)
+    if at is not None:
+        d["reset"].zero_(); d["reset"][at[0]] = 1
+        d["f"][at[1]] = float("nan")
+    else:
+        bad = [float("nan")] + ([float("inf"), -float("inf")] if infinite else [])
+        for x in (d["f"], d["x"], d["o"], dy):
+            if x is None:
+                continue
+            for _ in range(max(2, T * B * H // 150)):
+                x[r.randint(T), r.randint(B), r.randint(H)] = bad[r.randint(len(bad))]
+    w, wy = wide(d), f64(dy)
+    with np.errstate(invalid="ignore", over="ignore"):
+        y, _, _, h = Q.gated_scan(**w)
+        df, dx, do, dh0, _ = Q.gated_scan_grad(dy=wy, dh_last=f64(dh), **w)
+    clean = {k: None if v is None else torch.tensor(np.where(np.isfinite(f64(v)), f64(v), {"f": 100.0}.get(k, 0.0)) if v.is_floating_point() else f64(v)) for k, v in d.items()}
+    eh, _, delta, M = bounds(clean)
+    size = np.abs(np.where(np.isfinite(wy), wy, 0.0))
+    shut = dict(wide(clean), o=None, reset=None)
+    G = Q.gated_scan_grad(dy=size, dh_last=np.abs(f64(dh)), **shut)[4]
+    eg = bounds(clean, G)[1]
+    D = float(size.max())
+    gy, gh, save = engine.gated_scan(**d, keep=True)
+    out = engine.gated_scan_backward(d["f"], d["x"], dy, save, o=d["o"], h0=d["h0"], reset=d["reset"], lens=d["lens"], dh_last=dh)
+    seen = 0
+    for name, got, ref, tol, kind in (("y", gy, y, eh + 3 * U * M, t), ("h_last", gh, h, eh, "f32"), ("df", out[0], df, 0.25 * (2 * M * eg + G * 2 * eh) + 0.5 * M * G * (2 * delta + 8 * U), t),
+                                      ("dx", out[1], dx, eg + G * (delta + 8 * U), t), ("do", out[2], do, 0.25 * D * eh + 0.25 * D * M * (2 * delta + 8 * U), t), ("dh0", out[3], dh0, eg + 4 * U * max(G, 1.0), "f32")):
+        if ref is None:
+            assert got is None
+            continue
+        got, fine = f64(got), np.isfinite(ref)
+        assert np.array_equal(np.isfinite(got), fine), (name, "not finite at", np.argwhere(np.isfinite(got) != fine)[:5].tolist())
+        assert np.isnan(got[np.isnan(ref)]).all() or infinite, name
+        err = np.abs(got[fine] - ref[fine]) - half_step(kind) * np.abs(ref[fine]) * (1 + 1e-3) - smallest(kind)
+        assert err.size == 0 or err.max() <= tol, (name, float(err.max()), tol)
+        seen += int((~fine).sum())
+    assert seen > 0

@@ -366,3 +366,10 @@ def test_refusals_on_the_device(dev):
                  lambda: engine.AdamW([f]).step([torch.zeros(4, 2, 3)]), lambda: engine.AdamW([f, torch.zeros(3)])):
         with pytest.raises((ValueError, RuntimeError)):
             call()
+
+
+@pytest.mark.parametrize("case", [dict(T=24, B=1, H=2, at=(10, 12)), dict(T=300, B=1, H=2, at=(160, 165)), dict(T=300, B=1, H=2, at=(95, 97)), dict(T=400, B=9, H=64, gate=True, lens=True),
+                                  dict(T=33, B=70, H=40, t="bf16", infinite=True), dict(T=5000, B=2, H=33, t="f16", gate=True, infinite=True), dict(T=1500, B=3, H=64, lens=True)],
+                         ids=lambda c: "-".join("%s%s" % kv for kv in c.items()))
+def test_what_is_not_finite_passes_no_reset(dev, case):
+    S.check_not_finite(dev, **case)

@@ -259,3 +259,16 @@ def test_the_moments_noise_is_spread_evenly():
     lim = 5 * 0.5 / np.sqrt(n)
     for r in (a, a ^ b, a ^ c, a[1:] ^ a[:-1], a[256:] ^ a[:-256]):
         assert np.abs(bits(r).mean(0) - 0.5).max() < lim * 1.01
+
+
+NOT_FINITE = [
+    dict(T=24, B=1, H=2, at=(10, 12)), dict(T=24, B=1, H=2, at=(12, 10)), dict(T=24, B=1, H=2, at=(10, 10)), dict(T=40, B=1, H=3, at=(17, 22)), dict(T=40, B=1, H=3, at=(7, 8)),
+    dict(T=300, B=1, H=2, at=(160, 165)), dict(T=300, B=1, H=2, at=(95, 97)), dict(T=300, B=1, H=2, gate=True, at=(159, 160)),
+    dict(T=24, B=6, H=5, gate=True), dict(T=70, B=4, H=6, t="bf16"), dict(T=70, B=4, H=6, gate=True, lens=True, infinite=True), dict(T=300, B=3, H=6, gate=True, lens=True), dict(T=300, B=3, H=5, t="f16", infinite=True),
+    dict(T=1100, B=2, H=4, infinite=True),
+]
+
+
+@pytest.mark.parametrize("case", NOT_FINITE, ids=lambda c: "-".join("%s%s" % kv for kv in c.items()))
+def test_emulated_scan_what_is_not_finite_passes_no_reset(dev, case):  # noqa: F811
+    S.check_not_finite(dev, **case)
