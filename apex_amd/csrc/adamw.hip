@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(Table T, double* parts,
 }
 
 struct Hyper {
-    float beta1, omb1, beta2, omb2, eps, lr, grad_scale, max_norm;
+    float beta1, omb1, beta2, omb2, eps, lr, grad_scale, max_norm; double norm_scale;      // (f64 as the norm is: 1 / 3 in f32 moved it by 3e-8)
     const double* parts; int n_parts;      // 0: no clipping
     const Step* step; const int64_t* t; uint64_t seed; double* norm_out;
 };
@@ -118,7 +118,7 @@ __device__ __forceinline__ bool clip_factor(const Hyper& P, bool first, float& k
     if (P.n_parts == 0) return true;
     double s = 0;
     for (int i = threadIdx.x; i < P.n_parts; i += 256) s += P.parts[i];
-    const double norm = sqrt(block_sum(s)) * fabs((double)P.grad_scale);
+    const double norm = sqrt(block_sum(s)) * P.norm_scale;
     if (first && P.norm_out && threadIdx.x == 0) *P.norm_out = norm;
     const float c = P.max_norm / ((float)norm + 1e-6f);
     k = (c < 1.f ? c : 1.f) * P.grad_scale;
@@ -387,7 +387,7 @@ extern "C" int apx_adamw(const apx_adamw_args* a, void* stream) {
         hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(64), 0, s, a->t, W.step, a->lr, a->beta1, a->beta2);
         APX_LAUNCH_CHECK();
     }
-    const Hyper P = {(float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps, (float)a->lr, (float)a->grad_scale, (float)a->max_norm,
+    const Hyper P = {(float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps, (float)a->lr, (float)a->grad_scale, (float)a->max_norm, std::fabs(a->grad_scale),
                      W.parts, n_parts, W.step, a->t, a->seed, a->norm_out};
     Walk w = {0, 0, 0};
     for (bool first = true; next(w, T) || first; first = false) {      // (a set of empty tensors counts a step and has a norm of 0)

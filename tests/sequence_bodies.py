@@ -256,3 +256,14 @@ def check_not_finite(dev, T, B, H, t="f32", gate=False, lens=False, infinite=Fal
         assert err.size == 0 or err.max() <= tol, (name, float(err.max()), tol)
         seen += int((~fine).sum())
     assert seen > 0
+
+
+def check_adamw_scaled_norm(dev):
+    """norm is f64 throughout: |scale| sqrt(sum g^2) to 1e-12 whatever the scale (200 squares and their sum in f64: 200 x 2^-53)"""
+    from apex_amd import engine
+    g = torch.tensor(np.random.RandomState(0).randn(200), dtype=torch.float32).to(dev)
+    for scale in (1.0 / 3, -0.1, 1e30, 7e-20):
+        o = engine.AdamW([torch.zeros(200, device=dev)], max_norm=1.0)
+        o.step([g], grad_scale=scale)
+        N = Q.clip_factor([f64(g)], scale, 1.0)[0]
+        assert abs(float(o.norm) - N) <= 1e-12 * N, (scale, float(o.norm), N)

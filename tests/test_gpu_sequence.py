@@ -373,3 +373,7 @@ def test_refusals_on_the_device(dev):
                          ids=lambda c: "-".join("%s%s" % kv for kv in c.items()))
 def test_what_is_not_finite_passes_no_reset(dev, case):
     S.check_not_finite(dev, **case)
+
+
+def test_adamw_scaled_norm(dev):
+    S.check_adamw_scaled_norm(dev)

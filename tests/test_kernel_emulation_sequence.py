@@ -272,3 +272,7 @@ NOT_FINITE = [
 @pytest.mark.parametrize("case", NOT_FINITE, ids=lambda c: "-".join("%s%s" % kv for kv in c.items()))
 def test_emulated_scan_what_is_not_finite_passes_no_reset(dev, case):  # noqa: F811
     S.check_not_finite(dev, **case)
+
+
+def test_emulated_adamw_scaled_norm(dev):  # noqa: F811
+    S.check_adamw_scaled_norm(dev)
