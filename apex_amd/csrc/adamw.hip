@@ -112,9 +112,11 @@ struct Hyper {
     const double* parts; int n_parts;      // 0: no clipping
     const Step* step; const int64_t* t; uint64_t seed; double* norm_out;
 };
-// what the gradients are multiplied by; false: the norm is not finite
-__device__ __forceinline__ bool clip_factor(const Hyper& P, bool first, float& k) {
-    k = P.grad_scale;
+// What the gradients are multiplied by: k, and 2^-64 before it if `far`; false: the norm is not finite.  Far: the norm, the ratio or k is beyond f32's normal numbers (gradients of 1e37
+// in a thousand elements have a norm of 1e39); k is formed in f64 then and taken apart, exactly: a gradient that 2^-64 rounds gives a product below all f32 numbers.
+constexpr float LEAST = 1.17549435e-38f;      // the smallest normal number
+__device__ __forceinline__ bool clip_factor(const Hyper& P, bool first, float& k, bool& far) {
+    k = P.grad_scale; far = false;
     if (P.n_parts == 0) return true;
     double s = 0;
     for (int i = threadIdx.x; i < P.n_parts; i += 256) s += P.parts[i];
@@ -122,7 +124,17 @@ __device__ __forceinline__ bool clip_factor(const Hyper& P, bool first, float& k
     if (first && P.norm_out && threadIdx.x == 0) *P.norm_out = norm;
     const float c = P.max_norm / ((float)norm + 1e-6f);
     k = (c < 1.f ? c : 1.f) * P.grad_scale;
+    if (c < LEAST || fabsf(k) < LEAST) {
+        const double ratio = (double)P.max_norm / (norm + 1e-6), q = (ratio < 1.0 ? ratio : 1.0) * (double)P.grad_scale;
+        far = fabs(q) < 0x1p-62;
+        k = (float)(far ? q * 0x1p64 : q);
+    }
+    far = wave_uniform(far);
     return norm <= 1.7976931348623157e308;
+}
+__device__ __forceinline__ void nearer(float (&g)[2][4]) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) g[q >> 2][q & 3] *= 0x1p-64f;
 }
 __device__ __forceinline__ void adam(float g, float& m, float& v, float& p, const Hyper& P, const Step& S, float keep) {
     m = m * P.beta1 + g * P.omb1;
@@ -135,8 +147,8 @@ __device__ __forceinline__ void adam(float g, float& m, float& v, float& p, cons
 // 256 MB in front of the memory (ordinary accesses: 320 us for the update of such a network; so: 270 us, 5.6 TB/s with the gradients).
 template <int TYPE>
 __global__ __launch_bounds__(256) void adamw32_kernel(Table T, Hyper P, float* __restrict__ M, float* __restrict__ V) {
-    float c;      // what a gradient is multiplied by
-    if (!clip_factor(P, blockIdx.x == 0, c)) return;
+    float c; bool far;      // what a gradient is multiplied by
+    if (!clip_factor(P, blockIdx.x == 0, c, far)) return;
     const Step S = *P.step;
     for (int chunk = blockIdx.x; chunk < T.chunks; chunk += gridDim.x) {
         const int id = entry_of(T, chunk);
@@ -151,6 +163,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(Table T, Hyper P, float* _
                 load_grad<TYPE>(T.g[id], (int64_t)e0 + i, g[q]);
                 pp[q] = APX_PASSING((const F4*)(p + i)); mm[q] = APX_PASSING((const F4*)(m + i)); vv[q] = APX_PASSING((const F4*)(v + i));
             }
+            if (far) nearer(g);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 const int i = q * 1024 + threadIdx.x * 4;
@@ -163,7 +176,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(Table T, Hyper P, float* _
                 APX_PASS((F4*)(p + i), pp[q]); APX_PASS((F4*)(m + i), mm[q]); APX_PASS((F4*)(v + i), vv[q]);
             }
         } else {
-            for (unsigned i = threadIdx.x; i < left; i += 256) adam(grad_at<TYPE>(T.g[id], (int64_t)e0 + i) * c, m[i], v[i], p[i], P, S, keep);
+            for (unsigned i = threadIdx.x; i < left; i += 256) adam(grad_at<TYPE>(T.g[id], (int64_t)e0 + i) * (far ? 0x1p-64f : 1.f) * c, m[i], v[i], p[i], P, S, keep);
         }
     }
 }
@@ -224,8 +237,8 @@ __device__ __forceinline__ unsigned wave_top(unsigned x) {
 // f32 (scales are powers of two), the block's largest is found on the bits, so the same inputs give the same codes whatever the launch looks like.
 template <int TYPE>
 __global__ __launch_bounds__(256) void adamw8_kernel(Table T, Hyper P, uint8_t* __restrict__ M, uint8_t* __restrict__ V, float* __restrict__ MS, float* __restrict__ VS) {
-    float c;      // what a gradient is multiplied by
-    if (!clip_factor(P, blockIdx.x == 0, c)) return;
+    float c; bool far;      // what a gradient is multiplied by
+    if (!clip_factor(P, blockIdx.x == 0, c, far)) return;
     const Step S = *P.step;
     const unsigned key = step_key(P.seed, *P.t);
     const int wave = wave_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -250,6 +263,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Table T, Hyper P, uint8_t* 
             mm[q] = APX_PASSING((const C4*)(M + blk * BLOCK + lane * 4)); vv[q] = APX_PASSING((const C4*)(V + blk * BLOCK + lane * 4));
             ms[q] = MS[blk]; vs[q] = VS[blk];
         }
+        if (far) nearer(g);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const unsigned e = e0 + (q * 4 + wave) * BLOCK;

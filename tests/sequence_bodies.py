@@ -267,3 +267,32 @@ def check_adamw_scaled_norm(dev):
         o.step([g], grad_scale=scale)
         N = Q.clip_factor([f64(g)], scale, 1.0)[0]
         assert abs(float(o.norm) - N) <= 1e-12 * N, (scale, float(o.norm), N)
+
+
+def check_adamw_far_norms(dev):
+    """Norms beyond f32's range and factors below its normal numbers: N is finite in 64 bits, so k = scale min(1, max_norm / (N + 1e-6)) counts as it stands.  Zero moments, one step.
+    k: the norm, its sum with 1e-6, the division, scale and their product, each rounded to f32: 5u (where it is formed in f64: u).  k g: 6u.  m: (1 - beta1) and its product: 8u.
+    v: the square 2 x 6 + 1, (1 - beta2) and its product: 15u.  Half a step of the smallest numbers twice: 2^-149.  The update: m 8u, half of v's 15u, square root 2u, ibc and its product
+    2u, eps and its sum 2u, reciprocal 2u, its product u, lr / (1 - beta1) and its product 2u: 27u.  p: decay, its product and the difference: 3u of p (the decay's own roundings are
+    1e-4 of that)."""
+    from apex_amd import engine
+    r = np.random.RandomState(4)
+    for bits in (32, 8):
+        for size, max_norm, scale, n in ((3e37, 1.0, 1.0, 1000), (1e37, 1e-3, 1.0, 2500), (3e37, 1e-6, -0.5, 2049), (1e25, 2.0, 1e30, 300), (1e30, 1e-3, 1e10, 5000), (2e37, 3e38, 1.0, 3000), (1e-25, 1e-3, 1e38, 700)):
+            g = torch.tensor(r.randn(n) * size, dtype=torch.float32).clamp(-3.3e38, 3.3e38).to(dev)
+            p = torch.tensor(r.randn(n) * 0.1, dtype=torch.float32).to(dev)
+            p0, g64 = f64(p), f64(g)
+            o = engine.AdamW([p], lr=1e-3, eps=1e-8, weight_decay=0.1, max_norm=max_norm, state_bits=bits)
+            o.step([g], grad_scale=scale)
+            N, k = Q.clip_factor([g64], scale, float(np.float32(max_norm)))
+            assert np.isfinite(N) and abs(float(o.norm) - N) <= 1e-12 * N
+            want, m, v = Q.adamw(p0, g64, np.zeros(n), np.zeros(n), 1, 1e-3, 0.9, 0.999, 1e-8, 0.1, k)
+            what = (bits, size, max_norm, scale)
+            if bits == 32:
+                assert (np.abs(f64(o.m)[:n] - m) <= 8 * U * np.abs(m) + 2.0 ** -149).all(), what
+            if v.max() > 3e38:      # (clipped to a norm of 3e38 the squares are no f32 numbers any more)
+                continue
+            if bits == 32:
+                assert (np.abs(f64(o.v)[:n] - v) <= 15 * U * v + 2.0 ** -149).all(), what
+            tol = 3.001 * U * np.abs(p0).max() + 27 * U * np.abs(want - p0).max()
+            assert np.abs(f64(p) - want).max() <= tol, (what, np.abs(f64(p) - want).max(), tol)

@@ -377,3 +377,7 @@ def test_what_is_not_finite_passes_no_reset(dev, case):
 
 def test_adamw_scaled_norm(dev):
     S.check_adamw_scaled_norm(dev)
+
+
+def test_adamw_far_norms(dev):
+    S.check_adamw_far_norms(dev)

@@ -276,3 +276,7 @@ def test_emulated_scan_what_is_not_finite_passes_no_reset(dev, case):  # noqa: F
 
 def test_emulated_adamw_scaled_norm(dev):  # noqa: F811
     S.check_adamw_scaled_norm(dev)
+
+
+def test_emulated_adamw_far_norms(dev):  # noqa: F811
+    S.check_adamw_far_norms(dev)
