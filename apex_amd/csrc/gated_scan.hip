@@ -611,19 +611,27 @@ int check_common(const apx_gated_scan_args* a) {
     APX_REQUIRE(a, "args");
     APX_REQUIRE(a->type == APX_F32 || a->type == APX_BF16 || a->type == APX_F16, "type");
     APX_REQUIRE(sizes_fit(a->T, a->B, a->H), "T, B, H");
-    for (const void* p : {(const void*)a->h0, (const void*)a->lens, (const void*)a->h_last, (const void*)a->save, (const void*)a->dh_last, (const void*)a->dh0})
-        APX_REQUIRE(aligned(p, 4), "4-byte alignment");
     return APX_OK;
 }
-Scan scan_of(const apx_gated_scan_args* a) {
+// Only what the direction uses is looked at and handed on: a field that is not read may hold anything.
+Scan scan_of(const apx_gated_scan_args* a, bool back) {
     Scan S = {};
     S.T = a->T; S.B = a->B; S.H = a->H;
-    S.f = a->f; S.x = a->x; S.o = a->o; S.dy = a->dy; S.y = a->y; S.df = a->df; S.dx = a->dx; S.do_ = a->do_;
     const int64_t e = size_of(a->type);
-    S.sf = {a->f_t * e, a->f_b * e}; S.sx = {a->x_t * e, a->x_b * e}; S.so = {a->o_t * e, a->o_b * e}; S.sy = {a->y_t * e, a->y_b * e};
-    S.sdy = {a->dy_t * e, a->dy_b * e}; S.sdf = {a->df_t * e, a->df_b * e}; S.sdx = {a->dx_t * e, a->dx_b * e}; S.sdo = {a->do_t * e, a->do_b * e};
-    S.h0 = a->h0; S.dh_last = a->dh_last; S.h_last = a->h_last; S.save = a->save; S.dh0 = a->dh0;
-    S.reset = a->reset; S.lens = a->lens;
+    if (a->T > 0) {
+        S.f = a->f; S.sf = {a->f_t * e, a->f_b * e};
+        S.x = a->x; S.sx = {a->x_t * e, a->x_b * e};
+        if (a->o) { S.o = a->o; S.so = {a->o_t * e, a->o_b * e}; }
+        if (back) {
+            S.dy = a->dy; S.sdy = {a->dy_t * e, a->dy_b * e};
+            S.df = a->df; S.sdf = {a->df_t * e, a->df_b * e};
+            S.dx = a->dx; S.sdx = {a->dx_t * e, a->dx_b * e};
+            if (a->o) { S.do_ = a->do_; S.sdo = {a->do_t * e, a->do_b * e}; }
+        } else { S.y = a->y; S.sy = {a->y_t * e, a->y_b * e}; }
+        S.reset = a->reset; S.lens = a->lens; S.save = a->save;
+    }
+    if (back) { S.dh_last = a->dh_last; S.dh0 = a->dh0; }
+    else { S.h0 = a->h0; S.h_last = a->h_last; }
     return S;
 }
 
@@ -700,12 +708,13 @@ extern "C" int apx_gated_scan_forward(const apx_gated_scan_args* a, void* stream
     if (const int rc = check_common(a)) return rc;
     if (a->B == 0 || a->H == 0) return APX_OK;
     APX_REQUIRE(a->h_last && a->h_last != a->h0, "h_last is given and is not h0");
+    APX_REQUIRE(aligned(a->h0, 4) && aligned(a->h_last, 4) && aligned(a->lens, 4) && aligned(a->save, 4), "4-byte alignment");
     if (a->T > 0) {
         APX_SCAN_IN(f, f); APX_SCAN_IN(x, x); APX_SCAN_OUT(y, y);
         if (a->o) APX_SCAN_IN(o, o);
         APX_REQUIRE(a->y != a->f && a->y != a->x && a->y != a->o, "y must not lie on an input");
     }
-    Scan S = scan_of(a);
+    Scan S = scan_of(a, false);
     APX_SCAN_WORKSPACE();
     return run(a->type, S, false, a->workspace, (hipStream_t)stream);
 }
@@ -713,6 +722,7 @@ extern "C" int apx_gated_scan_forward(const apx_gated_scan_args* a, void* stream
 extern "C" int apx_gated_scan_backward(const apx_gated_scan_args* a, void* stream) {
     if (const int rc = check_common(a)) return rc;
     if (a->B == 0 || a->H == 0) return APX_OK;
+    APX_REQUIRE(aligned(a->h0, 4) && aligned(a->dh_last, 4) && aligned(a->dh0, 4) && aligned(a->lens, 4) && aligned(a->save, 4), "4-byte alignment");
     if (a->T > 0) {
         APX_SCAN_IN(f, f); APX_SCAN_IN(x, x); APX_SCAN_IN(dy, dy); APX_SCAN_OUT(df, df); APX_SCAN_OUT(dx, dx);
         if (a->o) { APX_SCAN_IN(o, o); APX_SCAN_OUT(do_, do); }
@@ -725,7 +735,7 @@ extern "C" int apx_gated_scan_backward(const apx_gated_scan_args* a, void* strea
     }
     APX_REQUIRE(!a->dh0 || a->dh0 != a->dh_last, "dh0 is not dh_last");
     if (a->T == 0 && !a->dh0) return APX_OK;
-    Scan S = scan_of(a);
+    Scan S = scan_of(a, true);
     APX_SCAN_WORKSPACE();
     return run(a->type, S, true, a->workspace, (hipStream_t)stream);
 }

@@ -280,3 +280,39 @@ def test_emulated_adamw_scaled_norm(dev):  # noqa: F811
 
 def test_emulated_adamw_far_norms(dev):  # noqa: F811
     S.check_adamw_far_norms(dev)
+
+
+def test_emulated_scan_leaves_unread_fields_alone(dev):  # noqa: F811
+    """fields that a call does not read may hold anything: odd and huge strides, pointers to nowhere (never followed), in both directions, without o, without steps, and for one step"""
+    from apex_amd import _lib, engine
+    lib = _lib.load()
+    T, B, H = 150, 3, 6
+    odd, huge, low = 0x7ffffffffffffff1, (1 << 62) + 3, -(1 << 62)
+    t = lambda *s: torch.randn(*s)  # noqa: E731
+    f, x, dy, h0 = t(T, B, H), t(T, B, H), t(T, B, H), t(B, H)
+    y, hl, df, dx = torch.zeros(T, B, H), torch.zeros(B, H), torch.zeros(T, B, H), torch.zeros(T, B, H)
+    ry, rh, save = engine.gated_scan(f, x, h0=h0, keep=True)
+    rdf, rdx, _, _ = engine.gated_scan_backward(f, x, dy, save, h0=h0)
+    st = lambda k: {k + "_t": B * H, k + "_b": H}  # noqa: E731
+    ws = torch.zeros(max(16, lib.apx_gated_scan_workspace_bytes(T, B, H)), dtype=torch.uint8)
+    base = dict(type=0, H=H, T=T, B=B, f=f.data_ptr(), x=x.data_ptr(), **st("f"), **st("x"), workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+    assert ws.data_ptr() % 16 == 0
+    for a, b in ((odd, huge), (low, low), (huge, odd)):
+        fwd = dict(base, y=y.data_ptr(), **st("y"), h0=h0.data_ptr(), h_last=hl.data_ptr(), o=0, o_t=a, o_b=b, dy=odd, dy_t=a, dy_b=b, df=odd, df_t=a, df_b=b, dx=odd, dx_t=a, dx_b=b, do_=odd, do_t=a,
+                   do_b=b, dh_last=odd, dh0=odd)
+        y.zero_(); hl.zero_()
+        assert lib.apx_gated_scan_forward(C.byref(_lib.GatedScanArgs(**fwd)), None) == 0, lib.apx_last_error()
+        assert torch.equal(y, ry) and torch.equal(hl, rh)
+        bwd = dict(base, dy=dy.data_ptr(), **st("dy"), df=df.data_ptr(), **st("df"), dx=dx.data_ptr(), **st("dx"), save=save.data_ptr(), y=odd, y_t=a, y_b=b, h_last=odd, o=0, o_t=a, o_b=b, do_=odd, do_t=a, do_b=b)
+        df.zero_(); dx.zero_()
+        assert lib.apx_gated_scan_backward(C.byref(_lib.GatedScanArgs(**bwd)), None) == 0, lib.apx_last_error()
+        assert torch.equal(df, rdf) and torch.equal(dx, rdx)
+        none = dict(type=0, H=H, T=0, B=B, f=odd, f_t=a, f_b=b, x=odd, x_t=a, x_b=b, y=odd, y_t=a, y_b=b, o=odd, o_t=a, o_b=b, h0=h0.data_ptr(), h_last=hl.data_ptr())
+        assert lib.apx_gated_scan_forward(C.byref(_lib.GatedScanArgs(**none)), None) == 0, lib.apx_last_error()
+        assert torch.equal(hl, h0)
+        h, y1 = h0.clone(), torch.zeros(B, H)
+        one = dict(type=0, H=H, T=-7, B=B, f=f.data_ptr(), f_t=a, f_b=H, x=x.data_ptr(), x_t=b, x_b=H, y=y1.data_ptr(), y_t=a, y_b=H, h0=odd, lens=odd, h_last=odd, save=odd, dy=odd, dy_t=a, dy_b=b, dh_last=odd,
+                   df=odd, dx=odd, do_=odd, dh0=odd, workspace=odd, workspace_bytes=3)
+        assert lib.apx_gated_scan_step(C.byref(_lib.GatedScanArgs(**one)), h.data_ptr(), None) == 0, lib.apx_last_error()
+        want = engine.gated_scan(f[:1], x[:1], h0=h0)
+        assert torch.equal(y1, want[0][0]) and torch.equal(h, want[1])
