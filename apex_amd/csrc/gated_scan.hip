@@ -594,6 +594,77 @@ bool reaches(int64_t T, int64_t B, int H, int64_t st, int64_t sb) {
     const __int128 last = (__int128)(T > 0 ? T - 1 : 0) * st + (__int128)(B > 0 ? B - 1 : 0) * sb + H;
     return st >= 0 && sb >= 0 && last < ((__int128)1 << 60);
 }
+// What an operand takes of memory: rows of `row` bytes, n[k] of them s[k] bytes apart along each of two axes (an axis of one row, or of the same row again, has none).
+struct Span { uintptr_t at; int64_t n[2], s[2], row; };
+Span span(const void* p, int64_t nt, int64_t st, int64_t nb, int64_t sb, int64_t row) {
+    Span a = {(uintptr_t)p, {nt, nb}, {st, sb}, row};
+    for (int k = 0; k < 2; ++k) if (a.n[k] <= 1 || a.s[k] == 0) { a.n[k] = 1; a.s[k] = 0; }
+    return a;
+}
+Span dense(const void* p, int64_t bytes) { return span(p, 1, 0, 1, 0, bytes); }
+uintptr_t behind(const Span& a) { return a.at + (a.n[0] - 1) * a.s[0] + (a.n[1] - 1) * a.s[1] + a.row; }
+int64_t floor_div(int64_t x, int64_t y) { return x / y - (x % y < 0); }
+// Do rows of a and b of the same strides share a byte?  The difference of their beginnings is i S + j s + r with numbers of steps i, j and |r| below a row's length; where S is more than
+// all that j s + r can be, and s more than r, two candidates for each are all there are.  -1: the strides are not the same, or not so far apart.
+int meets_alike(const Span& a, const Span& b) {
+    int64_t s[2];
+    for (int k = 0; k < 2; ++k) {
+        if (a.n[k] > 1 && b.n[k] > 1 && a.s[k] != b.s[k]) return -1;
+        s[k] = a.n[k] > 1 ? a.s[k] : b.s[k];
+    }
+    const int far = s[0] >= s[1] ? 0 : 1, near = 1 - far;
+    const int64_t row = a.row > b.row ? a.row : b.row, n = a.n[near] > b.n[near] ? a.n[near] : b.n[near], D = (int64_t)(b.at - a.at);
+    if ((s[near] && s[near] < row) || (s[far] && s[far] < (n - 1) * s[near] + row)) return -1;
+    const int64_t i0 = s[far] ? floor_div(D, s[far]) : 0;
+    for (int64_t i = i0; i <= i0 + (s[far] != 0); ++i) {
+        if (i < 1 - b.n[far] || i > a.n[far] - 1) continue;
+        const int64_t rest = D - i * s[far], j0 = s[near] ? floor_div(rest, s[near]) : 0;
+        for (int64_t j = j0; j <= j0 + (s[near] != 0); ++j) {
+            if (j < 1 - b.n[near] || j > a.n[near] - 1) continue;
+            const int64_t r = rest - j * s[near];
+            if (-b.row < r && r < a.row) return 1;
+        }
+    }
+    return 0;
+}
+// Does an output, whose own rows lie apart and thus follow one another, share a byte with [at, at + bytes)?  The last row that begins at or in front of `at` does, or the next one does.
+bool meets_row(const Span& out, uintptr_t at, int64_t bytes) {
+    const int far = out.s[0] >= out.s[1] ? 0 : 1, near = 1 - far;
+    const int64_t D = (int64_t)(at - out.at);
+    if (D < 0) return D + bytes > 0;
+    int64_t i = out.s[far] ? D / out.s[far] : 0;
+    if (i >= out.n[far]) i = out.n[far] - 1;
+    const int64_t rest = D - i * out.s[far];
+    int64_t j = out.s[near] ? rest / out.s[near] : 0;
+    if (j >= out.n[near]) j = out.n[near] - 1;
+    if (rest - j * out.s[near] < out.row) return true;
+    if (j + 1 < out.n[near]) return i * out.s[far] + (j + 1) * out.s[near] < D + bytes;
+    return i + 1 < out.n[far] && (i + 1) * out.s[far] < D + bytes;
+}
+// ... with another operand?  Exact where their strides are the same - slices of one buffer - or the other has few rows; else all rows on one pitch that keep to columns of their own are
+// apart, and what is left counts as sharing.
+bool meets(const Span& out, const Span& b) {
+    if (behind(out) <= b.at || behind(b) <= out.at) return false;
+    if (b.n[0] == 1 && b.n[1] == 1) return meets_row(out, b.at, b.row);
+    const int alike = meets_alike(out, b);
+    if (alike >= 0) return alike;
+    int64_t pitch = 0;
+    for (const Span* a : {&out, &b}) for (int k = 0; k < 2; ++k) for (int64_t y = a->s[k]; y; ) { const int64_t x = pitch; pitch = y; y = x % y; }
+    const int64_t D = (int64_t)(b.at - out.at), column = D - floor_div(D, pitch) * pitch;
+    if (column >= out.row && column + b.row <= pitch) return false;
+    if (b.n[0] > 4096 / b.n[1]) return true;
+    for (int64_t i = 0; i < b.n[0]; ++i) for (int64_t j = 0; j < b.n[1]; ++j) if (meets_row(out, b.at + i * b.s[0] + j * b.s[1], b.row)) return true;
+    return false;
+}
+// the operands of a call: outputs first
+struct Spans {
+    Span a[16]; int n = 0, outputs = 0;
+    void add(const Span& s) { a[n++] = s; }
+    bool apart() const {
+        for (int i = 0; i < outputs; ++i) for (int k = i + 1; k < n; ++k) if (meets(a[i], a[k])) return false;
+        return true;
+    }
+};
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 size_t size_of(int type) { return type == APX_F32 ? 4 : 2; }
 #define APX_SCAN_IN(p, s) APX_REQUIRE(a->p && aligned(a->p, size_of(a->type)) && reaches(a->T, a->B, a->H, a->s##_t, a->s##_b), "input pointer / strides")
@@ -633,6 +704,23 @@ Scan scan_of(const apx_gated_scan_args* a, bool back) {
     if (back) { S.dh_last = a->dh_last; S.dh0 = a->dh0; }
     else { S.h0 = a->h0; S.h_last = a->h_last; }
     return S;
+}
+
+Spans spans_of(const Scan& S, const apx_gated_scan_args* a, bool back) {
+    Spans all;
+    const int64_t row = S.H * (int64_t)size_of(a->type), state = S.B * S.H * 4;
+    auto operand = [&](const void* p, const Strides& st) { if (p) all.add(span(p, S.T, st.t, S.B, st.b, row)); };
+    auto flat = [&](const void* p, size_t bytes) { if (p && bytes) all.add(dense(p, (int64_t)bytes)); };
+    const size_t save = apx_gated_scan_save_floats(S.T, S.B, S.H) * 4;
+    if (back) { operand(S.df, S.sdf); operand(S.dx, S.sdx); operand(S.do_, S.sdo); flat(S.dh0, state); }
+    else { operand(S.y, S.sy); flat(S.h_last, state); flat(S.save, save); }
+    flat(a->workspace, apx_gated_scan_workspace_bytes(S.T, S.B, S.H));
+    all.outputs = all.n;
+    operand(S.f, S.sf); operand(S.x, S.sx); operand(S.o, S.so);
+    if (back) { operand(S.dy, S.sdy); flat(S.save, save); flat(S.dh_last, state); }
+    else flat(S.h0, state);
+    flat(S.reset, S.T * S.B); flat(S.lens, S.B * 4);
+    return all;
 }
 
 // ------------------------------------------------------------------------------------------------ launches
@@ -707,15 +795,15 @@ extern "C" size_t apx_gated_scan_workspace_bytes(int64_t T, int64_t B, int H) {
 extern "C" int apx_gated_scan_forward(const apx_gated_scan_args* a, void* stream) {
     if (const int rc = check_common(a)) return rc;
     if (a->B == 0 || a->H == 0) return APX_OK;
-    APX_REQUIRE(a->h_last && a->h_last != a->h0, "h_last is given and is not h0");
+    APX_REQUIRE(a->h_last, "h_last");
     APX_REQUIRE(aligned(a->h0, 4) && aligned(a->h_last, 4) && aligned(a->lens, 4) && aligned(a->save, 4), "4-byte alignment");
     if (a->T > 0) {
         APX_SCAN_IN(f, f); APX_SCAN_IN(x, x); APX_SCAN_OUT(y, y);
         if (a->o) APX_SCAN_IN(o, o);
-        APX_REQUIRE(a->y != a->f && a->y != a->x && a->y != a->o, "y must not lie on an input");
     }
     Scan S = scan_of(a, false);
     APX_SCAN_WORKSPACE();
+    APX_REQUIRE(spans_of(S, a, false).apart(), "an output overlaps an input or another output");
     return run(a->type, S, false, a->workspace, (hipStream_t)stream);
 }
 
@@ -727,16 +815,11 @@ extern "C" int apx_gated_scan_backward(const apx_gated_scan_args* a, void* strea
         APX_SCAN_IN(f, f); APX_SCAN_IN(x, x); APX_SCAN_IN(dy, dy); APX_SCAN_OUT(df, df); APX_SCAN_OUT(dx, dx);
         if (a->o) { APX_SCAN_IN(o, o); APX_SCAN_OUT(do_, do); }
         APX_REQUIRE(a->save, "save of the forward call");
-        const void *in[4] = {a->f, a->x, a->dy, a->o}, *out[3] = {a->df, a->dx, a->o ? a->do_ : nullptr};
-        for (int i = 0; i < 3; ++i) {
-            for (int k = 0; k < 4; ++k) APX_REQUIRE(!out[i] || out[i] != in[k], "an output must not lie on an input");
-            for (int k = 0; k < i; ++k) APX_REQUIRE(!out[i] || out[i] != out[k], "outputs must not lie on each other");
-        }
     }
-    APX_REQUIRE(!a->dh0 || a->dh0 != a->dh_last, "dh0 is not dh_last");
     if (a->T == 0 && !a->dh0) return APX_OK;
     Scan S = scan_of(a, true);
     APX_SCAN_WORKSPACE();
+    APX_REQUIRE(spans_of(S, a, true).apart(), "an output overlaps an input or another output");
     return run(a->type, S, true, a->workspace, (hipStream_t)stream);
 }
 
@@ -750,8 +833,15 @@ extern "C" int apx_gated_scan_step(const apx_gated_scan_args* a, float* h, void*
     APX_REQUIRE(h && aligned(h, 4) && a->B * a->H < ((int64_t)1 << 31), "h, B * H");
     APX_SCAN_IN(f, f); APX_SCAN_IN(x, x); APX_SCAN_OUT(y, y);
     if (a->o) APX_SCAN_IN(o, o);
-    APX_REQUIRE(a->y != a->f && a->y != a->x && a->y != a->o && a->y != (const void*)h, "y must not lie on an input or on h");
-    const int64_t e = size_of(a->type);
+    const int64_t e = size_of(a->type), row = a->H * e;
+    Spans all;
+    all.add(span(a->y, 1, 0, a->B, a->y_b * e, row)); all.add(dense(h, a->B * a->H * 4));
+    all.outputs = 2;
+    // (h itself as an input - an element is read where it is written - is served)
+    auto input = [&](const void* p, int64_t sb) { if (p && !(p == h && a->type == APX_F32 && (a->B == 1 || sb == a->H))) all.add(span(p, 1, 0, a->B, sb * e, row)); };
+    input(a->f, a->f_b); input(a->x, a->x_b); input(a->o, a->o_b);
+    if (a->reset) all.add(dense(a->reset, a->B));
+    APX_REQUIRE(all.apart(), "y or h overlaps an input or the other");
     const OneStep S = {a->f, a->x, a->o, a->y, a->f_b * e, a->x_b * e, a->o_b * e, a->y_b * e, a->reset, (unsigned)(a->B * a->H), (unsigned)a->H};
     APX_BY_TYPE(a->type, gated_scan_step_kernel, apx_cdiv(a->B * a->H, 256), 256, (hipStream_t)stream, S, h);
     return APX_OK;

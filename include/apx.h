@@ -132,7 +132,8 @@ int apx_lstm_backward(const float* params, float* grads, int D, int H, int L, in
  *                          backward pass needs.
  * apx_gated_scan_backward: the inputs and save of a forward call, dy and dh_last (NULL = 0) -> df, dx, do_ (with o), dh0 (NULL = not wanted).
  * f, x, o, y, dy, df, dx, do_ hold `type` and lie as strides say, in elements: entry (t, b, j) at t * s_t + b * s_b + j, so f | x | o side by side in the rows of one
- * product need no copy.  Inputs may overlap or repeat (stride 0); outputs must not overlap each other or an input, nor themselves.  h0, h_last, save, dh_last, dh0: f32,
+ * product need no copy.  Inputs may overlap or repeat (stride 0); a call whose outputs overlap each other, an input or the workspace, or themselves, is refused (slices of one buffer that
+ * keep apart are taken; operands of more than 4096 rows whose strides do not show that they keep apart are refused too).  h0, h_last, save, dh_last, dh0: f32,
  * dense [B, H].  reset: u8, dense [T, B].  lens: i32 [B], below 0 taken as 0 and above T as T.  States, gates and sums are f32 whatever the type; each output is rounded once.
  * workspace: apx_gated_scan_workspace_bytes bytes (0 for most shapes: then it may be NULL), 16-byte aligned, not shared by calls that may run at the same time.
  * Every pointer is aligned to its own type.  Eight neighbouring steps of the sequences that share 128 channels (64 where H is odd) lie within 4 GB in every operand (T = 1: those
@@ -167,7 +168,8 @@ size_t apx_gated_scan_workspace_bytes(int64_t T, int64_t B, int H);
 int apx_gated_scan_forward(const apx_gated_scan_args* args, void* stream);
 int apx_gated_scan_backward(const apx_gated_scan_args* args, void* stream);
 /* One step of the same recurrence, for the rollout: h [B, H] f32 (dense) is updated in place, y [B, H] = the step's output; rows of f, x, o, y lie f_b, x_b, o_b, y_b
- * elements apart; rows whose reset byte ([B]) is non-zero start from a zero state.  T, lens, save and the backward fields are not read. */
+ * elements apart; rows whose reset byte ([B]) is non-zero start from a zero state.  T, lens, save and the backward fields are not read.
+ * y and h must not overlap each other or an input; h itself may be an f32 input. */
 int apx_gated_scan_step(const apx_gated_scan_args* args, float* h, void* stream);
 
 /* The padded minibatch of the recurrent update (rl/algos/ppo.py:411-430: pad_sequence over the sampled trajectories, zero rows behind a trajectory's end) gathered out of

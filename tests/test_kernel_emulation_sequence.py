@@ -316,3 +316,76 @@ def test_emulated_scan_leaves_unread_fields_alone(dev):  # noqa: F811
         assert lib.apx_gated_scan_step(C.byref(_lib.GatedScanArgs(**one)), h.data_ptr(), None) == 0, lib.apx_last_error()
         want = engine.gated_scan(f[:1], x[:1], h0=h0)
         assert torch.equal(y1, want[0][0]) and torch.equal(h, want[1])
+
+
+def test_emulated_scan_refuses_operands_that_overlap(dev):  # noqa: F811
+    """outputs shifted by one step, one sequence or one unit from an input or from each other are refused, slices of one buffer that keep apart are taken and give the same results"""
+    from apex_amd import engine
+    T, B, H = 6, 4, 5
+    buf = lambda *s: torch.randn(*s)  # noqa: E731
+    f, x, dy = buf(T, B, H), buf(T, B, H), buf(T, B, H)
+    ry, _, save = engine.gated_scan(f, x, keep=True)
+    rdf, rdx, _, _ = engine.gated_scan_backward(f, x, dy, save)
+
+    def into(view, t):
+        view.copy_(t)
+        return view
+
+    for make, cuts in ((lambda: buf(T + 1, B, H), (slice(0, T), slice(1, T + 1))), (lambda: buf(T, B + 1, H), ((slice(None), slice(0, B)), (slice(None), slice(1, B + 1)))),
+                       (lambda: buf(T, B, H + 1), ((Ellipsis, slice(0, H)), (Ellipsis, slice(1, H + 1)))), (lambda: buf(T, B, 2 * H - 1), ((Ellipsis, slice(0, H)), (Ellipsis, slice(H - 1, 2 * H - 1))))):
+        for a, b in (cuts, cuts[::-1]):
+            big = make()
+            for call in (lambda: engine.gated_scan(into(big[a], f), x, out=big[b]), lambda: engine.gated_scan(f, into(big[a], x), out=big[b]), lambda: engine.gated_scan(f, x, o=into(big[a], f), out=big[b]),
+                         lambda: engine.gated_scan_backward(f, x, into(big[a], dy), save, out=(big[b], torch.empty(T, B, H))), lambda: engine.gated_scan_backward(f, x, dy, save, out=(big[a], big[b])),
+                         lambda: engine.gated_scan(f, into(big[a], x), o=x, out=big[b])):
+                with pytest.raises(RuntimeError, match="overlap"):
+                    call()
+    for make, cuts in ((lambda: buf(2 * T, B, H), (slice(0, T), slice(T, 2 * T))), (lambda: buf(2 * T, B, H), (slice(0, 2 * T, 2), slice(1, 2 * T, 2))), (lambda: buf(T, 2 * B, H), ((slice(None), slice(0, 2 * B, 2)), (slice(None), slice(1, 2 * B, 2)))),
+                       (lambda: buf(T, B, 2 * H), ((Ellipsis, slice(0, H)), (Ellipsis, slice(H, 2 * H)))), (lambda: buf(B, T, 2 * H).permute(1, 0, 2), ((Ellipsis, slice(H, 2 * H)), (Ellipsis, slice(0, H))))):
+        big = make()
+        y, _ = engine.gated_scan(into(big[cuts[0]], f), x, out=big[cuts[1]])
+        assert torch.equal(y, ry)
+        df, dx, _, _ = engine.gated_scan_backward(f, x, dy, save, out=(big[cuts[0]], big[cuts[1]]))
+        assert torch.equal(df, rdf) and torch.equal(dx, rdx)
+    row = buf(T, B, 2 * H)      # one row for all steps, in columns of its own of the buffer that the output lies in
+    one = row[0, 1, H:].expand(T, B, H)
+    assert torch.equal(engine.gated_scan(f, one, out=row[..., :H])[0], engine.gated_scan(f, one.clone())[0])
+    h = torch.randn(B, H); want = h.clone()      # h as an input of its own step
+    y = engine.gated_scan_step(f[0], h, h)
+    z = engine.gated_scan_step(f[0], want.clone(), want)
+    assert torch.equal(h, want) and torch.equal(y, z)
+    with pytest.raises(RuntimeError, match="overlap"):
+        engine.gated_scan_step(f[0], x[0], h, out=h)
+
+
+def test_emulated_scan_overlaps_by_chance(dev):  # noqa: F811
+    """600 layouts in a small buffer: a call is refused exactly where its output shares a byte with an input (bytes counted one by one), else it gives what separate buffers give"""
+    from apex_amd import _lib, engine
+    lib = _lib.load()
+    r = np.random.RandomState(0)
+    refused = taken = 0
+    while refused + taken < 600:
+        T, B, H = r.randint(1, 5), r.randint(1, 5), r.randint(1, 5)
+        near = H + r.randint(0, 9); far = (max(T, B) - 1) * near + H + r.randint(0, 9)
+        ys = (far, near) if r.rand() < 0.5 else (near, far)
+        fs = ys if r.rand() < 0.4 else tuple(int(r.choice([0, near, far, r.randint(0, 40)])) for _ in range(2))
+        size = 3 * far * 5 + 64
+        y0, f0, s0 = (int(r.randint(0, size // 3)) for _ in range(3))
+        place = lambda at, st: {at + t * st[0] + b * st[1] + j for t in range(T) for b in range(B) for j in range(H)}  # noqa: E731
+        mem = torch.randn(size)
+        Y, F, S0 = place(y0, ys), place(f0, fs), set(range(s0, s0 + B * H))
+        f = mem.as_strided((T, B, H), (*fs, 1), f0).clone(); h0 = mem[s0:s0 + B * H].view(B, H).clone()
+        x, hl = torch.randn(T, B, H), torch.zeros(B, H)
+        p = mem.data_ptr()
+        args = dict(type=0, H=H, T=T, B=B, f=p + 4 * f0, f_t=fs[0], f_b=fs[1], x=x.data_ptr(), x_t=B * H, x_b=H, y=p + 4 * y0, y_t=ys[0], y_b=ys[1], h0=p + 4 * s0, h_last=hl.data_ptr())
+        before = mem.clone()
+        rc = lib.apx_gated_scan_forward(C.byref(_lib.GatedScanArgs(**args)), None)
+        if Y & F or Y & S0:
+            assert rc == -1 and b"overlap" in lib.apx_last_error() and torch.equal(mem, before), (T, B, H, ys, fs, y0, f0, s0)
+            refused += 1
+        else:
+            assert rc == 0, (T, B, H, ys, fs, y0, f0, s0, lib.apx_last_error())
+            ry, rh = engine.gated_scan(f, x, h0=h0)
+            assert torch.equal(mem.as_strided((T, B, H), (*ys, 1), y0), ry) and torch.equal(hl, rh)
+            taken += 1
+    assert min(refused, taken) > 100
