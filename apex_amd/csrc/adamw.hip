@@ -11,7 +11,10 @@
 // Products and sums of the moments are separate roundings (no fused multiply-add), so that the moments are the same numbers wherever the formula above is evaluated in f32.
 #include "apx_common.h"
 #include <gfx950/half_types.h>
+#include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 
 namespace {
 
@@ -326,6 +329,43 @@ int64_t entries_of(int n_tensors, const int64_t* numel) {
 // (one even where there is nothing: it counts the step)
 int launches_of(int n_tensors, const int64_t* numel) { const int64_t k = entries_of(n_tensors, numel); return k ? (int)((k + TABLE - 1) / TABLE) : 1; }
 
+// Does nothing that a step writes - parameters, moments, count, norm, workspace - share memory with anything else that it writes, or with a gradient?  (Gradients may be the same ones.)
+// Pieces in the order of their addresses, which sets of tensors mostly have anyway: one walk, 1 us for 200 tensors.
+struct Piece { uintptr_t from, to; };
+bool operator<(const Piece& a, const Piece& b) { return a.from < b.from; }
+Piece* in_order(Piece* a, int n) {
+    if (!std::is_sorted(a, a + n)) std::sort(a, a + n);
+    return a + n;
+}
+int apart(const apx_adamw_args* a, int64_t elements, size_t workspace) {
+    constexpr int FEW = 256;
+    Piece few[3 * FEW + 16], rest[8];
+    std::unique_ptr<Piece[]> many(a->n_tensors > FEW ? new (std::nothrow) Piece[3 * (size_t)a->n_tensors + 16] : nullptr);
+    if (a->n_tensors > FEW && !many) { apx_set_error("apx_adamw: no memory to check %d tensors", a->n_tensors); return APX_E_ARG; }
+    Piece* const g = many ? many.get() : few, * const p = g + a->n_tensors, * const w = p + a->n_tensors;
+    int ng = 0, np = 0, nr = 0;
+    auto piece = [](const void* at, int64_t bytes) { return Piece{(uintptr_t)at, (uintptr_t)at + (uintptr_t)bytes}; };
+    for (int i = 0; i < a->n_tensors; ++i) {
+        if (a->numel[i] == 0) continue;
+        p[np++] = piece(a->params[i], a->numel[i] * 4);
+        g[ng++] = piece(a->grads[i], a->numel[i] * (a->grad_type == APX_F32 ? 4 : 2));
+    }
+    auto add = [&](const void* at, int64_t bytes) { if (at && bytes) rest[nr++] = piece(at, bytes); };
+    const int64_t code = a->state_bits == 32 ? 4 : 1;
+    add(a->m, elements * code); add(a->v, elements * code);
+    if (a->state_bits == 8) { add(a->m_scale, elements / BLOCK * 4); add(a->v_scale, elements / BLOCK * 4); }
+    add(a->t, 8); add(a->norm_out, 8); add(a->workspace, (int64_t)workspace);
+    in_order(g, ng);
+    Piece* const end = std::merge(p, in_order(p, np), rest, in_order(rest, nr), w);
+    for (Piece* x = w; x + 1 < end; ++x) APX_REQUIRE(x->to <= x[1].from, "two of the parameters, moments, t, norm_out and workspace overlap");
+    const Piece* x = w;
+    for (int i = 0; i < ng; ++i) {
+        while (x < end && x->to <= g[i].from) ++x;
+        APX_REQUIRE(x == end || x->from >= g[i].to, "a gradient lies on what the step writes");
+    }
+    return APX_OK;
+}
+
 }  // namespace
 
 #define APX_BY_TYPE(type, kernel, grid, block, s, ...)                                                                    \
@@ -363,7 +403,9 @@ extern "C" int apx_adamw(const apx_adamw_args* a, void* stream) {
     APX_REQUIRE(total < ((int64_t)1 << 39), "numel in all");
     APX_REQUIRE(total == 0 || (a->m && a->v && (a->state_bits == 32 || (a->m_scale && a->v_scale))), "moments");
     APX_REQUIRE((((uintptr_t)a->m | (uintptr_t)a->v | (uintptr_t)a->m_scale | (uintptr_t)a->v_scale) & 3) == 0, "moments: 4-byte alignment");
-    APX_REQUIRE(a->workspace && ((uintptr_t)a->workspace & 15) == 0 && a->workspace_bytes >= apx_adamw_workspace_bytes(a->n_tensors, a->numel), "workspace");
+    const size_t need = apx_adamw_workspace_bytes(a->n_tensors, a->numel);
+    APX_REQUIRE(a->workspace && ((uintptr_t)a->workspace & 15) == 0 && a->workspace_bytes >= need, "workspace");
+    if (const int rc = apart(a, apx_adamw_state_elements(a->n_tensors, a->numel), need)) return rc;
     const hipStream_t s = (hipStream_t)stream;
     const Workspace W = workspace_of(a->workspace);
     const bool clip = a->max_norm > 0;
@@ -419,6 +461,10 @@ extern "C" int apx_adamw_moments(const void* m, const void* v, const float* m_sc
     if (elements == 0) return APX_OK;
     APX_REQUIRE(m && v && m_scale && v_scale && m_out && v_out, "null pointer");
     APX_REQUIRE((((uintptr_t)m_scale | (uintptr_t)v_scale) & 3) == 0 && (((uintptr_t)m | (uintptr_t)v) & 7) == 0 && (((uintptr_t)m_out | (uintptr_t)v_out) & 15) == 0, "alignment");
+    const Piece io[6] = {{(uintptr_t)m_out, (uintptr_t)m_out + 2 * (uintptr_t)elements}, {(uintptr_t)v_out, (uintptr_t)v_out + 2 * (uintptr_t)elements},
+                         {(uintptr_t)m, (uintptr_t)m + (uintptr_t)elements}, {(uintptr_t)v, (uintptr_t)v + (uintptr_t)elements},
+                         {(uintptr_t)m_scale, (uintptr_t)m_scale + (uintptr_t)(elements / BLOCK * 4)}, {(uintptr_t)v_scale, (uintptr_t)v_scale + (uintptr_t)(elements / BLOCK * 4)}};
+    for (int i = 0; i < 2; ++i) for (int k = i + 1; k < 6; ++k) APX_REQUIRE(io[i].to <= io[k].from || io[k].to <= io[i].from, "an output overlaps an input or the other output");
     const int64_t want = (elements + 2047) / 2048;
     hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)(want < GRID ? want : GRID)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)m, (const uint8_t*)v, m_scale, v_scale,
                        elements, (uint16_t*)m_out, (uint16_t*)v_out);

@@ -390,7 +390,7 @@ class AdamW:
         self._index, self._shapes = self.params[0].get_device(), [p.shape for p in self.params]
         self._held = [p.detach() for p in self.params]      # (keeps the memory that the pointers below name)
         self._pointers = [p.data_ptr() for p in self.params]
-        self._ps, self._taken = array.array("Q", self._pointers), {p.data_ptr() for p in self.params if p.numel()}
+        self._ps = array.array("Q", self._pointers)
         self._args = _lib.AdamwArgs(n_tensors=n, state_bits=state_bits, params=self._ps.buffer_info()[0], numel=C.addressof(self._numel), weight_decay=C.addressof(self._decay),
                                     m=_p(self.m), v=_p(self.v), m_scale=_p(self.m_scale), v_scale=_p(self.v_scale), t=_p(self.t), workspace=_p(self._ws),
                                     workspace_bytes=self._ws.numel(), norm_out=_p(self.norm))
@@ -418,10 +418,7 @@ class AdamW:
             raise ValueError("a tensor of params has moved since this optimiser was made: it works on the memory that it was given")
         if index >= 0 and index != torch._C._cuda_getDevice():
             return _elsewhere(self.step, index, grads, grad_scale, lr)
-        gs = list(map(torch.Tensor.data_ptr, grads))
-        if not self._taken.isdisjoint(gs):
-            raise ValueError("a gradient lies on a tensor of params")
-        gs = array.array("Q", gs)
+        gs = array.array("Q", map(torch.Tensor.data_ptr, grads))
         if self.max_norm is not None and not self.max_norm > 0:
             raise ValueError("max_norm is %r, expected a positive number or None" % (self.max_norm,))
         a = self._args

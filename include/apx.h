@@ -278,8 +278,8 @@ int apx_clip_adam(float* param, float* m, float* v, float* grad, int64_t n, floa
  * max_norm <= 0: no clipping (k = grad_scale, N is not formed, norm_out is not written).  With clipping a step whose N is infinite or NaN changes neither parameters nor
  * moments (t still counts it); norm_out shows it.
  * 0 <= beta < 1, eps > 0 (a normal f32: the update of a moment that is still 0 is 0, not 0 / 0).
- * params / grads / numel / weight_decay: [host] arrays of n_tensors entries (weight_decay NULL: 0); the tensors dense, parameters f32, gradients grad_type.  Tensors must not
- * overlap.  Empty tensors are allowed.
+ * params / grads / numel / weight_decay: [host] arrays of n_tensors entries (weight_decay NULL: 0); the tensors dense, parameters f32, gradients grad_type.  Tensors that
+ * overlap each other, a gradient on what the step writes, and outputs of apx_adamw_moments on its inputs are refused; gradients may repeat.  Empty tensors are allowed.
  * Moments: one flat block each for m and v, in the tensors' order, every tensor's part starting at a multiple of 256 elements (apx_adamw_state_elements in all); zero before
  * the first step.  state_bits 32: f32.  state_bits 8: one u8 code per element and one f32 scale per 256 elements of a tensor (m_scale, v_scale), a power of two s >= 2^-94 with
  * max|.| in [s, 2 s), or below s = 2^-94.  An m code is a sign bit above a 7-bit c, a v code an 8-bit c; c stands for 0 if c = 0, else for s times the f32 number with the bits (c + 904) << 20 (m)

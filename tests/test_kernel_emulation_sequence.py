@@ -389,3 +389,50 @@ def test_emulated_scan_overlaps_by_chance(dev):  # noqa: F811
             assert torch.equal(mem.as_strided((T, B, H), (*ys, 1), y0), ry) and torch.equal(hl, rh)
             taken += 1
     assert min(refused, taken) > 100
+
+
+def test_emulated_adamw_refuses_memory_that_overlaps(dev):  # noqa: F811
+    """a gradient that reaches into a parameter, a moment or another part of the state, and parameters or state that overlap, are refused and nothing changes; neighbours are taken"""
+    from apex_amd import _lib, engine
+    lib = _lib.load()
+    n = 600
+    block = torch.randn(4 * n)
+    for order in (1, -1):
+        for many in (1, 300):      # (more than the table on the stack holds, in ascending and descending order)
+            ps = [torch.randn(3) for _ in range(many - 1)][::order] + [block[n:2 * n]]
+            o = engine.AdamW(ps, state_bits=32)
+            gs = [torch.randn(3) for _ in range(many - 1)]
+            start = block.clone()
+            for at in (1, n - 1, n + 1, 2 * n - 1):
+                with pytest.raises(RuntimeError, match="gradient"):
+                    o.step(gs + [block[at:at + n]])
+            for bad in (o.m[:n], o.v[5:n + 5]):
+                with pytest.raises(RuntimeError, match="gradient"):
+                    o.step(gs + [bad])
+            assert torch.equal(block, start) and int(o.t) == 0 and not o.m.any()
+            o.step(gs + [block[:n]]); o.step(gs + [block[2 * n:3 * n]])
+            assert int(o.t) == 2 and torch.equal(block[:n], start[:n]) and torch.equal(block[2 * n:], start[2 * n:])
+    g, q = torch.randn(4), [torch.zeros(4), torch.zeros(4)]
+    o = engine.AdamW(q)
+    o.step([g, g])
+    assert torch.equal(q[0], q[1]) and q[0].any()
+
+    p, m, v, ws, t, norm = torch.randn(600), torch.zeros(1024), torch.zeros(1024), torch.zeros(20000, dtype=torch.uint8), torch.zeros(2, dtype=torch.int64), torch.zeros(1, dtype=torch.float64)
+    g = torch.randn(600)
+
+    def step(**change):
+        ptr, grad, num = (C.c_void_p * 2)(p.data_ptr(), p.data_ptr() + 4 * change.pop("second", 300)), (C.c_void_p * 2)(g.data_ptr(), g.data_ptr()), (C.c_int64 * 2)(300, 300)
+        a = dict(n_tensors=2, grad_type=0, state_bits=32, params=C.addressof(ptr), grads=C.addressof(grad), numel=C.addressof(num), m=m.data_ptr(), v=v.data_ptr(), t=t.data_ptr(), lr=1e-3, beta1=0.9,
+                 beta2=0.999, eps=1e-8, grad_scale=1.0, max_norm=1.0, workspace=ws.data_ptr(), workspace_bytes=ws.numel(), norm_out=norm.data_ptr())
+        return lib.apx_adamw(C.byref(_lib.AdamwArgs(**{**a, **change})), None)
+    before = p.clone()
+    for change in (dict(second=299), dict(second=0), dict(m=v.data_ptr()), dict(v=m.data_ptr() + 4 * 1023), dict(t=norm.data_ptr()), dict(norm_out=ws.data_ptr() + 8), dict(t=m.data_ptr() + 8),
+                   dict(m=p.data_ptr()), dict(v=g.data_ptr()), dict(norm_out=p.data_ptr() + 8)):
+        assert step(**change) == -1 and any(w in lib.apx_last_error() for w in (b"overlap", b"lies on")), change
+        assert torch.equal(p, before) and int(t[0]) == 0
+    assert step() == 0 and int(t[0]) == 1 and not torch.equal(p, before)
+    c, s, out = torch.zeros(1024, dtype=torch.uint8), torch.ones(8), torch.zeros(4096, dtype=torch.uint8)
+    assert out.data_ptr() % 16 == 0 and c.data_ptr() % 16 == 0
+    mom = lambda mo, vo: lib.apx_adamw_moments(c.data_ptr(), c.data_ptr() + 512, s.data_ptr(), s.data_ptr() + 8, 512, mo, vo, None)  # noqa: E731
+    assert [mom(c.data_ptr(), out.data_ptr()), mom(out.data_ptr(), c.data_ptr() + 512), mom(out.data_ptr(), out.data_ptr() + 1008)] == [-1] * 3 and b"overlap" in lib.apx_last_error()
+    assert mom(out.data_ptr(), out.data_ptr() + 1024) == 0
