@@ -23,6 +23,7 @@ using namespace half_types;
 constexpr int TABLE = 120;                 // entries a launch: 32 bytes each, of 4 kB of kernel arguments
 constexpr int BLOCK = 256;                 // elements that share a scale of 8-bit moments, and what a tensor's part of the moments is rounded up to
 constexpr int CHUNK = 2048;                // elements a workgroup takes at a time: 8 blocks, 8 elements a thread
+constexpr int64_t LARGEST = (int64_t)1 << 39;     // elements of a tensor, and of all
 constexpr int64_t ENTRY = (int64_t)1 << 31;      // elements of an entry: a larger tensor takes several
 constexpr int PARTS = 1024;                // partial sums of squares of one launch (512 or 2048: 77 and 80 us instead of 73)
 constexpr int GRID = 4096;                 // workgroups of the update at most: 16 for each of 256 CUs (8 for each: 335 instead of 323 us, 32 for each: 8-bit moments 5 % slower)
@@ -321,13 +322,14 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const uint8_t* __res
 
 struct Workspace { Step* step; double* parts; };
 Workspace workspace_of(void* w) { return {(Step*)w, (double*)((char*)w + 64)}; }
-int64_t entries_of(int n_tensors, const int64_t* numel) {
+// `numel` in whole pieces of `by` elements a tensor; sizes that a step refuses count for none
+int64_t pieces_of(int n_tensors, const int64_t* numel, int64_t by) {
     int64_t k = 0;
-    for (int i = 0; i < n_tensors; ++i) k += numel[i] > 0 ? (numel[i] + ENTRY - 1) / ENTRY : 0;
+    for (int i = 0; numel && i < n_tensors; ++i) k += numel[i] > 0 && numel[i] < LARGEST ? (numel[i] + by - 1) / by : 0;
     return k;
 }
 // (one even where there is nothing: it counts the step)
-int launches_of(int n_tensors, const int64_t* numel) { const int64_t k = entries_of(n_tensors, numel); return k ? (int)((k + TABLE - 1) / TABLE) : 1; }
+int launches_of(int n_tensors, const int64_t* numel) { const int64_t k = pieces_of(n_tensors, numel, ENTRY); return k ? (int)((k + TABLE - 1) / TABLE) : 1; }
 
 // Does nothing that a step writes - parameters, moments, count, norm, workspace - share memory with anything else that it writes, or with a gradient?  (Gradients may be the same ones.)
 // Pieces in the order of their addresses, which sets of tensors mostly have anyway: one walk, 1 us for 200 tensors.
@@ -377,9 +379,7 @@ int apart(const apx_adamw_args* a, int64_t elements, size_t workspace) {
     } while (0)
 
 extern "C" int64_t apx_adamw_state_elements(int n_tensors, const int64_t* numel) {
-    int64_t n = 0;
-    for (int i = 0; i < n_tensors; ++i) n += numel[i] > 0 ? (numel[i] + BLOCK - 1) / BLOCK * BLOCK : 0;
-    return n;
+    return pieces_of(n_tensors, numel, BLOCK) * BLOCK;
 }
 extern "C" size_t apx_adamw_workspace_bytes(int n_tensors, const int64_t* numel) { return 64 + (size_t)launches_of(n_tensors, numel) * PARTS * sizeof(double); }
 
@@ -394,13 +394,13 @@ extern "C" int apx_adamw(const apx_adamw_args* a, void* stream) {
     APX_REQUIRE((float)a->eps >= 1.17549435e-38f && std::isfinite((float)a->eps) && std::isfinite((float)a->lr) && std::isfinite((float)a->grad_scale) && !std::isnan(a->max_norm), "eps, lr, grad_scale, max_norm");
     int64_t total = 0;
     for (int i = 0; i < a->n_tensors; ++i) {
-        APX_REQUIRE(a->numel[i] >= 0 && a->numel[i] < ((int64_t)1 << 39), "numel");
+        APX_REQUIRE(a->numel[i] >= 0 && a->numel[i] < LARGEST, "numel");
         APX_REQUIRE(a->numel[i] == 0 || (a->params[i] && a->grads[i]), "null tensor");
         APX_REQUIRE(a->numel[i] == 0 || (((uintptr_t)a->params[i] & 3) == 0 && ((uintptr_t)a->grads[i] & (a->grad_type == APX_F32 ? 3 : 1)) == 0), "tensor alignment");
         APX_REQUIRE(!a->weight_decay || std::isfinite(a->weight_decay[i]), "weight_decay");
         total += a->numel[i];
+        APX_REQUIRE(total < LARGEST, "numel in all");
     }
-    APX_REQUIRE(total < ((int64_t)1 << 39), "numel in all");
     APX_REQUIRE(total == 0 || (a->m && a->v && (a->state_bits == 32 || (a->m_scale && a->v_scale))), "moments");
     APX_REQUIRE((((uintptr_t)a->m | (uintptr_t)a->v | (uintptr_t)a->m_scale | (uintptr_t)a->v_scale) & 3) == 0, "moments: 4-byte alignment");
     const size_t need = apx_adamw_workspace_bytes(a->n_tensors, a->numel);

@@ -436,3 +436,13 @@ def test_emulated_adamw_refuses_memory_that_overlaps(dev):  # noqa: F811
     mom = lambda mo, vo: lib.apx_adamw_moments(c.data_ptr(), c.data_ptr() + 512, s.data_ptr(), s.data_ptr() + 8, 512, mo, vo, None)  # noqa: E731
     assert [mom(c.data_ptr(), out.data_ptr()), mom(out.data_ptr(), c.data_ptr() + 512), mom(out.data_ptr(), out.data_ptr() + 1008)] == [-1] * 3 and b"overlap" in lib.apx_last_error()
     assert mom(out.data_ptr(), out.data_ptr() + 1024) == 0
+
+
+def test_adamw_sizes_of_no_tensors():
+    """the two size functions follow no NULL and count nothing for sizes that a step refuses"""
+    from apex_amd import _lib
+    lib = _lib.load()
+    none = lib.apx_adamw_workspace_bytes(0, None)
+    assert none >= 64 + 8 and lib.apx_adamw_workspace_bytes(3, None) == none and lib.apx_adamw_state_elements(3, None) == 0 and lib.apx_adamw_state_elements(-1, None) == 0
+    num = (C.c_int64 * 4)(-5, 1 << 39, (1 << 63) - 1, 3)
+    assert lib.apx_adamw_state_elements(4, num) == 256 and lib.apx_adamw_workspace_bytes(4, num) == none
