@@ -17,8 +17,9 @@ def _p(t):
 
 
 def _stream():
-    """The current stream of the current device (its handle alone: the Stream object of torch.cuda.current_stream() costs 3 us of host time a call)."""
-    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+    """The current stream of the current device (its handle alone: the Stream object of torch.cuda.current_stream() costs 3 us of host time a call).  current_device() initialises torch's
+    side as current_stream() does, and raises where that would, in a forked child for instance."""
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _need_gpu(*ts):

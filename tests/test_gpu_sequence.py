@@ -381,3 +381,18 @@ def test_adamw_scaled_norm(dev):
 
 def test_adamw_far_norms(dev):
     S.check_adamw_far_norms(dev)
+
+
+def test_the_stream_is_torchs(dev):
+    """the handle that the calls are launched on is that of torch.cuda.current_stream(), on the default stream, on another and inside a capture"""
+    from apex_amd import engine
+    same = lambda: (engine._stream().value or 0) == torch.cuda.current_stream().cuda_stream  # noqa: E731
+    side = torch.cuda.Stream()
+    assert same()
+    with torch.cuda.stream(side):
+        assert same() and engine._stream().value == side.cuda_stream
+    graph, f = torch.cuda.CUDAGraph(), torch.zeros(2, 3, device=dev)
+    with torch.cuda.graph(graph):
+        assert same()
+        f.add_(1)
+    assert same()

@@ -446,3 +446,15 @@ def test_adamw_sizes_of_no_tensors():
     assert none >= 64 + 8 and lib.apx_adamw_workspace_bytes(3, None) == none and lib.apx_adamw_state_elements(3, None) == 0 and lib.apx_adamw_state_elements(-1, None) == 0
     num = (C.c_int64 * 4)(-5, 1 << 39, (1 << 63) - 1, 3)
     assert lib.apx_adamw_state_elements(4, num) == 256 and lib.apx_adamw_workspace_bytes(4, num) == none
+
+
+def test_the_stream_of_a_forked_process_is_refused(monkeypatch):
+    """engine._stream() passes torch's own lazy initialisation: what torch.cuda.current_stream() refuses - a child forked from a process that uses the GPU - is refused with torch's message"""
+    from apex_amd import engine
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)      # (what such a child would otherwise be told)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda k: 0, raising=False)
+    monkeypatch.setattr(torch.cuda, "_initialized", True)
+    assert engine._stream().value is None      # the default stream's handle
+    monkeypatch.setattr(torch.cuda, "_is_in_bad_fork", lambda: True)
+    with pytest.raises(RuntimeError, match="fork"):
+        engine._stream()
