@@ -296,3 +296,31 @@ def check_adamw_far_norms(dev):
                 assert (np.abs(f64(o.v)[:n] - v) <= 15 * U * v + 2.0 ** -149).all(), what
             tol = 3.001 * U * np.abs(p0).max() + 27 * U * np.abs(want - p0).max()
             assert np.abs(f64(p) - want).max() <= tol, (what, np.abs(f64(p) - want).max(), tol)
+
+
+def check_adamw_decays(dev, count, bits, clip, grad="f32", steps=3):
+    """Tensors of a few sizes, more of them than one launch takes, each with a decay of its own between 0.1 and 1 at lr 1e-2: a step takes 1e-3 to 1e-2 of a parameter away, against a bound of
+    some 1e-6 for EACH tensor, kept by itself over the steps.  Per step: 3u |p| (decay, its product, the difference; the decay's own roundings 2u of a hundredth: 0.02u more), and of the
+    update 27u + 3u a step before (check_adamw_far_norms; m and v bring 3u more from every step)."""
+    from apex_amd import engine
+    r = np.random.RandomState(count)
+    shapes = [(1 + k % 5, 1 + k % 3) for k in range(count)]
+    ps = [torch.tensor(r.randn(*s), dtype=torch.float32).to(dev) for s in shapes]
+    decay = [0.1 + 0.9 * ((7 * k) % count) / count for k in range(count)]
+    hyper = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-5)
+    opt = engine.AdamW(ps, weight_decay=decay, max_norm=clip, state_bits=bits, **hyper)
+    P, M, V, spread = [f64(p) for p in ps], [np.zeros(s) for s in shapes], [np.zeros(s) for s in shapes], np.zeros(count)
+    for t in range(1, steps + 1):
+        g = [torch.tensor(r.randn(*s), dtype=torch.float32).to(NP[grad]).to(dev) for s in shapes]
+        opt.step(g)
+        k = Q.clip_factor([f64(x) for x in g], 1.0, clip)[1]
+        moments = [(f64(a), f64(b)) for a, b in zip(opt.views(opt.moments()[0]), opt.views(opt.moments()[1]))]
+        for i in range(count):
+            p, M[i], V[i] = Q.adamw(P[i], f64(g[i]), M[i], V[i], t, hyper["lr"], *hyper["betas"], hyper["eps"], float(np.float32(decay[i])), k)
+            if bits == 8:
+                M[i], V[i] = moments[i]      # (what the next step begins with; this step's update uses the moments before their rounding)
+            spread[i] += 3.02 * U * np.abs(P[i]).max() + (27 + 3 * t) * U * np.abs(p - P[i] * (1 - hyper["lr"] * decay[i])).max()
+            err = np.abs(f64(ps[i]) - p).max()
+            assert err <= spread[i], (i, t, err, spread[i])
+            assert spread[i] < 0.01 * hyper["lr"] * 0.1 * np.abs(P[i]).max() or np.abs(P[i]).max() < 0.1, "the bound does not tell a decay from none"
+            P[i] = p
