@@ -324,3 +324,29 @@ def check_adamw_decays(dev, count, bits, clip, grad="f32", steps=3):
             assert err <= spread[i], (i, t, err, spread[i])
             assert spread[i] < 0.01 * hyper["lr"] * 0.1 * np.abs(P[i]).max() or np.abs(P[i]).max() < 0.1, "the bound does not tell a decay from none"
             P[i] = p
+
+
+def check_adamw_eight_bits_over_many_steps(dev, n, steps):
+    """8-bit against 32-bit moments over the same gradients, N(1/2, 1) times 1e-2, steps of them.
+    v: every rounding keeps the mean, so E v8 = v32.  With s = E g^2 and D = E (v8 - v32)^2: the rounding of what moved by d off the grid has a variance of at most |d| times the grid's step, at
+    most v8 / 8, and d = (1 - b2) (g^2 - v8) with g independent of v8: D' <= b2^2 D + (1 - b2) / 8 (s v8 + v8^2) in the mean <= b2^2 D + (1 - b2) / 8 ((2 + e) s^2 + D), e = the variance of v32
+    in s^2, below 0.01: D <= (2 + e) / 8 / (1 + b2 - 1 / 8) s^2 = 0.135 s^2 at every step.  The means of n elements: five standard deviations of 0.367 / sqrt(n) for v8 - v32, and 0.05 for its
+    square (a fourth moment of 10 D^2 gives 5 x 3 x 0.135 / sqrt(1024) = 0.063 at the fewest elements used; taken as 0.07).
+    p: m8's rounding is independent of v8's and keeps the mean; 1 / sqrt(v8) is above 1 / sqrt(v32) in the mean (convexity), to second order by 3/8 x 0.135 = 0.05; twice that is allowed above,
+    and for the means of n displacements five of their own standard errors either way."""
+    from apex_amd import engine
+    r = np.random.RandomState(n)
+    size, b2 = 1e-2, 0.999
+    p8, p32 = (torch.zeros(n, device=dev) for _ in range(2))
+    o8, o32 = engine.AdamW([p8], lr=1e-3, betas=(0.9, b2), eps=1e-8, state_bits=8, seed=3), engine.AdamW([p32], lr=1e-3, betas=(0.9, b2), eps=1e-8)
+    for _ in range(steps):
+        g = torch.tensor((0.5 + r.randn(n)) * size, dtype=torch.float32).to(dev)
+        o8.step([g]); o32.step([g])
+    s = 1.25 * size * size
+    off = (f64(o8.moments()[1])[:n] - f64(o32.v)[:n]) / s
+    assert abs(off.mean()) <= 5 * 0.367 / np.sqrt(n), off.mean()
+    assert (off ** 2).mean() <= 0.135 + 0.07, (off ** 2).mean()
+    a, b = -f64(p8), -f64(p32)
+    room = 5 * np.sqrt(a.var() / n + b.var() / n)
+    assert b.mean() > 0 and b.mean() - room <= a.mean() <= 1.1 * b.mean() + room, (a.mean(), b.mean(), room)
+    return off, a, b

@@ -401,3 +401,8 @@ def test_the_stream_is_torchs(dev):
 @pytest.mark.parametrize("case", [dict(count=130, bits=32, clip=0.05), dict(count=250, bits=8, clip=None), dict(count=121, bits=32, clip=None, grad="bf16"), dict(count=500, bits=8, clip=1.0, grad="f16")], ids=str)
 def test_adamw_every_tensor_has_its_decay(dev, case):
     S.check_adamw_decays(dev, **case)
+
+
+@pytest.mark.parametrize("n,steps", [(1 << 16, 300), (5000, 3000)])
+def test_adamw_eight_bits_over_many_steps(dev, n, steps):
+    S.check_adamw_eight_bits_over_many_steps(dev, n, steps)

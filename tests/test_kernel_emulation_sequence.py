@@ -463,3 +463,7 @@ def test_the_stream_of_a_forked_process_is_refused(monkeypatch):
 @pytest.mark.parametrize("case", [dict(count=130, bits=32, clip=0.05), dict(count=250, bits=8, clip=None), dict(count=121, bits=32, clip=None, grad="bf16"), dict(count=119, bits=8, clip=1.0)], ids=str)
 def test_emulated_adamw_every_tensor_has_its_decay(dev, case):  # noqa: F811
     S.check_adamw_decays(dev, **case)
+
+
+def test_emulated_adamw_eight_bits_over_many_steps(dev):  # noqa: F811
+    S.check_adamw_eight_bits_over_many_steps(dev, 1024, 300)
