@@ -281,7 +281,8 @@ def gated_scan(f, x, o=None, h0=None, reset=None, lens=None, keep=False, out=Non
     """The gated linear recurrence h_t = sigmoid(f_t) h_{t-1} + sigmoid(-f_t) x_t over [T, B, H] (f32, bf16 or f16; any strides with the units of a row next to each other, so
     slices of one product's rows need no copy).  y = h, or h sigmoid(o).  h0 [B, H] f32 = the carried state (None: zero); reset [T, B] uint8: a non-zero byte starts that step
     from a zero state (an episode start); lens [B] int32: steps from lens[b] on are padding - the state stays and y is 0 there.  out: where y goes (it must not lie on an input).
-    Returns (y [T, B, H], h_last [B, H] f32), with keep=True (y, h_last, save) for gated_scan_backward.  States, gates and sums are f32 whatever the type."""
+    Returns (y [T, B, H], h_last [B, H] f32), with keep=True (y, h_last, save) for gated_scan_backward.  States, gates and sums are f32 whatever the type.
+    Like every call of this module it is unknown to autograd: results carry no graph, also where an input requires gradients; those are gated_scan_backward's."""
     head, dev, held = _scan_inputs(f, x, o, h0, reset, lens)
     if dev >= 0 and dev != torch._C._cuda_getDevice():
         return _elsewhere(gated_scan, dev, f, x, o, h0, reset, lens, keep, out)
@@ -324,7 +325,7 @@ def gated_scan_backward(f, x, dy, save, o=None, h0=None, reset=None, lens=None, 
 
 def gated_scan_step(f, x, h, o=None, reset=None, out=None):
     """One step of gated_scan for a rollout: f, x, o [B, H], the carried state h [B, H] f32 updated in place (rows whose reset byte, uint8 [B], is non-zero start from zero);
-    returns y [B, H]."""
+    returns y [B, H].  Unknown to autograd (gated_scan)."""
     dev, shape, dtype = f.get_device(), f.shape, f.dtype
     if dev < 0:
         _need_gpu(f)
@@ -402,7 +403,8 @@ class AdamW:
     t = property(lambda self: self._t); norm = property(lambda self: self._norm)
 
     def step(self, grads, grad_scale=1.0, lr=None):
-        """One step on `grads`: one dense tensor for each of params (all f32, all bf16 or all f16), multiplied by grad_scale first (1 / world size of a summed gradient)."""
+        """One step on `grads`: one dense tensor for each of params (all f32, all bf16 or all f16), multiplied by grad_scale first (1 / world size of a summed gradient).
+        The parameters are written behind autograd's back: a graph that was recorded with their old values does not notice (as with .data)."""
         n, index = len(self.params), self._index
         if len(grads) != n:
             raise ValueError("%d gradients for %d tensors" % (len(grads), n))
