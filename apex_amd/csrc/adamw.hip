@@ -6,8 +6,8 @@
 // up again in every workgroup - a few kB out of L2, cheaper than a third launch - and makes the step.  Tensors go into the launches by tables in the kernel arguments
 // (no device copy of pointers that would have to be kept in step with the caller's): up to TABLE tensors a launch.
 // What bounds it: memory for large networks - 28 bytes a parameter with 32-bit moments, 12 + 4 with 8-bit ones, the gradients twice with a clip -, the launches for small ones.
-// Measured on an MI355X, 63 M parameters: norm 38 - 70 us (gradients in the caches or not: 3.6 TB/s, what a sum reads at), update 270 us (32 bits, f32 gradients), 160 us (8 bits, bf16
-// gradients, 5.5 TB/s); the 450 k parameters of a recurrent actor and critic: 3.8 + 5.8 us.
+// Measured on an MI355X, 63 M parameters: norm 38 - 70 us (gradients in the caches or not: 3.6 TB/s, what a sum reads at), update 273 us (32 bits, f32 gradients), 168 us (8 bits, bf16
+// gradients, 5.3 TB/s); the 450 k parameters of a recurrent actor and critic: 3.8 + 6.2 us.
 // Products and sums of the moments are separate roundings (no fused multiply-add), so that the moments are the same numbers wherever the formula above is evaluated in f32.
 #include "apx_common.h"
 #include <gfx950/half_types.h>
@@ -148,7 +148,7 @@ __device__ __forceinline__ void adam(float g, float& m, float& v, float& p, cons
 }
 
 // Parameters and moments pass by the caches: nobody reads them again soon, and 63 M parameters' 750 MB would drive out the gradients, which the norm has just brought into the
-// 256 MB in front of the memory (ordinary accesses: 320 us for the update of such a network; so: 270 us, 5.6 TB/s with the gradients).
+// 256 MB in front of the memory (ordinary accesses: 320 us for the update of such a network; so: 273 us).
 template <int TYPE>
 __global__ __launch_bounds__(256) void adamw32_kernel(Table T, Hyper P, float* __restrict__ M, float* __restrict__ V) {
     float c; bool far;      // what a gradient is multiplied by
@@ -332,7 +332,7 @@ int64_t pieces_of(int n_tensors, const int64_t* numel, int64_t by) {
 int launches_of(int n_tensors, const int64_t* numel) { const int64_t k = pieces_of(n_tensors, numel, ENTRY); return k ? (int)((k + TABLE - 1) / TABLE) : 1; }
 
 // Does nothing that a step writes - parameters, moments, count, norm, workspace - share memory with anything else that it writes, or with a gradient?  (Gradients may be the same ones.)
-// Pieces in the order of their addresses, which sets of tensors mostly have anyway: one walk, 1 us for 200 tensors.
+// Pieces in the order of their addresses, which sets of tensors mostly have anyway: one walk (a call with 200 tensors takes the host as long as one that only compared base pointers).
 struct Piece { uintptr_t from, to; };
 bool operator<(const Piece& a, const Piece& b) { return a.from < b.from; }
 Piece* in_order(Piece* a, int n) {

@@ -8,11 +8,13 @@
 // states), and the steps between are run again from there.
 //
 // What bounds it: memory.  Forward f, x (o) in, y out; backward f, x, dy (o) in, df, dx (do) out: 3 to 7 elements moved for some 45 to 90 vector instructions, so f32 runs at the
-// rate of a copy (5.0 TB/s on this card) and 16-bit types are near the rate at which the vector units issue.  Measured on an MI355X, kernel times:
-//   forward  f32  [400, 1024, 128], resets            124 us   5.1 TB/s        bf16 [32, 4096, 256], resets             39 us   5.2 TB/s
-//   backward f32  [400, 1024, 128], output gate       305 us   4.8 TB/s        bf16 [32, 4096, 256], resets             79 us   4.2 TB/s
-//   the same f32 pair with lengths of 1 .. 400 (half of the rows are padding and are not read): forward 129 us, backward 246 us
-//   forward  bf16 [16384, 4, 256], output gate: maps 15 us + scan 26 us; f32 [65536, 1, 128]: maps 13 + 20 us, backward maps 13 + 29 us (the split reads f and x or dy twice)
+// rate of a copy (5.0 TB/s on this card) and 16-bit types are near the rate at which the vector units issue.  Measured on an MI355X, kernel times
+// (medians of 23 launches):
+//   forward  f32  [400, 1024, 128], resets            124 us   5.1 TB/s        bf16 [32, 4096, 256], resets             44 us   4.8 TB/s
+//   backward f32  [400, 1024, 128], output gate       321 us   4.6 TB/s        bf16 [32, 4096, 256], resets             80 us   4.4 TB/s
+//   f32 with the output gate, forward 182 us; the pair with lengths of 1 .. 400 (half of the rows are padding and are not read): forward 131 us, backward 252 us
+//   forward  bf16 [16384, 4, 256], output gate: maps 15 us + scan 27 us; f32 [65536, 1, 128]: maps 15 + 21 us, backward maps 15 + 30.5 us (the split reads f and x or dy twice)
+//   f32 [65536, 1, 8] to [65536, 1, 64]: 11 + 16 to 17 us and 11 + 23 to 25 us, where the bytes take 1 to 8 us: lanes are channels, and below 128 of them a wave's others idle
 #include "apx_common.h"
 #include <gfx950/dynamic_lds.h>
 #include <gfx950/half_types.h>
@@ -44,12 +46,12 @@ template <> struct Elem<APX_F16> {
 constexpr int STEPS = 8;
 constexpr int WAVES = 8;                  // waves of a workgroup at most
 constexpr int KEEP = 32;                  // steps between two kept states; what a tile begins with is one of them
-// Channels of a lane: 2 where H is even (no pair lies across two sequences then).  One channel: bf16 [32, 4096, 256] forward 45 us against 39, backward 94 against 79, f32 the same.
+// Channels of a lane: 2 where H is even (no pair lies across two sequences then).  One channel: bf16 [32, 4096, 256] forward 49 us against 45, backward 97 against 80, f32 the same.
 // Four need more registers than there are for enough waves: bf16 backward 125 us.
 constexpr int VECTOR = 2;
 // The time axis is split into parts where there are SPLIT steps and the channels make fewer than FILL / 2 workgroups: f16 [333, 37, 100] took 30 us forward and 55 us backward
-// in one part (29 workgroups) and takes 13 and 18 in six.  FILL workgroups are then wanted: 768 or 1024 made bf16 [16384, 4, 256] 10 % slower, 256 made it 15 % slower.
-// SEGMENTS parts at most, because each folds the maps of all before it: 512 made the backward pass of f32 [65536, 1, 128] 40 us instead of 29.
+// in one part (29 workgroups) and takes 14 and 20 in six.  FILL workgroups are then wanted: 768 or 1024 made bf16 [16384, 4, 256] 10 % slower, 256 made it 15 % slower.
+// SEGMENTS parts at most, because each folds the maps of all before it: 512 made the backward pass of f32 [65536, 1, 128] 40 us instead of 31.
 constexpr int SPLIT = 128, FILL = 512, SEGMENTS = 256;
 constexpr int FOLD = 16;                  // maps of other parts that a wave has on their way at once (4: 4 us of the 21 to 30 us of a long scan's second pass; 32: registers)
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -410,7 +412,7 @@ __global__ __launch_bounds__(64 * WAVES) void gated_scan_fwd_kernel(Scan S) {
 // ------------------------------------------------------------------------------------------------ backward
 // The same walk from the end.  A tile begins with a kept state; the waves' maps of h (forward in time) and of c (backward: the same product of gates) meet in LDS together.  A wave
 // then runs its steps forward for the states and backward for the gradients, on registers alone.  (f32 without an output gate needs 183 of them, with one 229: 2 waves a SIMD,
-// enough for the memory.  Held to 128 by the launch bounds the compiler spills: 700 us for 305.  The output gate is evaluated twice rather than kept.)
+// enough for the memory.  Held to 128 by the launch bounds the compiler spills: 700 us for 321.  The output gate is evaluated twice rather than kept.)
 template <int TYPE, int VEC, bool GATE>
 __global__ __launch_bounds__(64 * WAVES) void gated_scan_bwd_kernel(Scan S) {
     typedef Row<TYPE, VEC> R;

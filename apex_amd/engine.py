@@ -354,7 +354,7 @@ class AdamW:
     """AdamW (decoupled weight decay) over the f32 tensors `params`, wherever they lie - the views of a flat parameter block, for instance -, behind a global-norm clip over all of
     their gradients (max_norm None: no clipping).  weight_decay: one number, or one for each tensor.  state_bits 32 keeps the moments in f32, 8 in 8 bits with a scale for every 256
     elements (include/apx.h, apx_adamw); seed names the pseudo-random bits that round those.  The step count lives on the device, so a captured step() counts when it is
-    replayed.  m, v (and m_scale, v_scale), t: the state, for a checkpoint.  norm [1] f64: the gradients' norm of the last clipped step - if it is infinite or NaN the step has
+    replayed (lr, scale, max_norm, seed and the gradients' addresses are those of the capture).  m, v (and m_scale, v_scale), t: the state, for a checkpoint.  norm [1] f64: the gradients' norm of the last clipped step - if it is infinite or NaN the step has
     changed nothing but t."""
 
     def __init__(self, params, lr=1e-4, betas=(0.9, 0.999), eps=1e-5, weight_decay=0.0, max_norm=None, state_bits=32, seed=0):

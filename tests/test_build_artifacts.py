@@ -245,7 +245,7 @@ def test_instruction_mix_ceilings_of_the_hot_env_kernels():
 
 
 def test_sequence_kernels_registers(code_objects):
-    """The gated scan's and AdamW's kernels keep everything in registers (no scratch, no spilled vector register: held to 128 registers the scan's f32 backward kernel takes 700 us instead of 305) and few enough of
+    """The gated scan's and AdamW's kernels keep everything in registers (no scratch, no spilled vector register: held to 128 registers the scan's f32 backward kernel takes 700 us instead of 321) and few enough of
     them for the waves that their times stand on: scan forward 4 waves a SIMD (128), backward 2 (256), in 16 bits without an output gate 3 (168), maps 3, AdamW 8 (64).  None of the packed
     f32 instructions that the build turns off for them."""
     seen = {}
