@@ -629,7 +629,12 @@ int meets_alike(const Span& a, const Span& b) {
     }
     return 0;
 }
-// Does an output, whose own rows lie apart and thus follow one another, share a byte with [at, at + bytes)?  The last row that begins at or in front of `at` does, or the next one does.
+// rows that lie apart and thus follow one another
+bool in_a_row(const Span& a) {
+    const int far = a.s[0] >= a.s[1] ? 0 : 1, near = 1 - far;
+    return (a.s[near] == 0 || a.s[near] >= a.row) && (a.s[far] == 0 || a.s[far] >= (a.n[near] - 1) * a.s[near] + a.row);
+}
+// Does an operand whose rows follow one another share a byte with [at, at + bytes)?  The last row that begins at or in front of `at` does, or the next one does.
 bool meets_row(const Span& out, uintptr_t at, int64_t bytes) {
     const int far = out.s[0] >= out.s[1] ? 0 : 1, near = 1 - far;
     const int64_t D = (int64_t)(at - out.at);
@@ -648,6 +653,7 @@ bool meets_row(const Span& out, uintptr_t at, int64_t bytes) {
 bool meets(const Span& out, const Span& b) {
     if (behind(out) <= b.at || behind(b) <= out.at) return false;
     if (b.n[0] == 1 && b.n[1] == 1) return meets_row(out, b.at, b.row);
+    if (out.n[0] == 1 && out.n[1] == 1 && in_a_row(b)) return meets_row(b, out.at, out.row);
     const int alike = meets_alike(out, b);
     if (alike >= 0) return alike;
     int64_t pitch = 0;
@@ -839,9 +845,9 @@ extern "C" int apx_gated_scan_step(const apx_gated_scan_args* a, float* h, void*
     Spans all;
     all.add(span(a->y, 1, 0, a->B, a->y_b * e, row)); all.add(dense(h, a->B * a->H * 4));
     all.outputs = 2;
-    // (h itself as an input - an element is read where it is written - is served)
-    auto input = [&](const void* p, int64_t sb) { if (p && !(p == h && a->type == APX_F32 && (a->B == 1 || sb == a->H))) all.add(span(p, 1, 0, a->B, sb * e, row)); };
-    input(a->f, a->f_b); input(a->x, a->x_b); input(a->o, a->o_b);
+    // (h itself as f or x is served: what is written is made of what was read there; o is read behind that)
+    auto input = [&](const void* p, int64_t sb, bool first) { if (p && !(first && p == h && a->type == APX_F32 && (a->B == 1 || sb == a->H))) all.add(span(p, 1, 0, a->B, sb * e, row)); };
+    input(a->f, a->f_b, true); input(a->x, a->x_b, true); input(a->o, a->o_b, false);
     if (a->reset) all.add(dense(a->reset, a->B));
     APX_REQUIRE(all.apart(), "y or h overlaps an input or the other");
     const OneStep S = {a->f, a->x, a->o, a->y, a->f_b * e, a->x_b * e, a->o_b * e, a->y_b * e, a->reset, (unsigned)(a->B * a->H), (unsigned)a->H};

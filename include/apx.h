@@ -169,7 +169,7 @@ int apx_gated_scan_forward(const apx_gated_scan_args* args, void* stream);
 int apx_gated_scan_backward(const apx_gated_scan_args* args, void* stream);
 /* One step of the same recurrence, for the rollout: h [B, H] f32 (dense) is updated in place, y [B, H] = the step's output; rows of f, x, o, y lie f_b, x_b, o_b, y_b
  * elements apart; rows whose reset byte ([B]) is non-zero start from a zero state.  T, lens, save and the backward fields are not read.
- * y and h must not overlap each other or an input; h itself may be an f32 input. */
+ * y and h must not overlap each other or an input; h itself may be f or x in f32. */
 int apx_gated_scan_step(const apx_gated_scan_args* args, float* h, void* stream);
 
 /* The padded minibatch of the recurrent update (rl/algos/ppo.py:411-430: pad_sequence over the sampled trajectories, zero rows behind a trajectory's end) gathered out of

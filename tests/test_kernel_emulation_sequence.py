@@ -467,3 +467,28 @@ def test_emulated_adamw_every_tensor_has_its_decay(dev, case):  # noqa: F811
 
 def test_emulated_adamw_eight_bits_over_many_steps(dev):  # noqa: F811
     S.check_adamw_eight_bits_over_many_steps(dev, 1024, 300)
+
+
+def test_emulated_scan_dense_outputs_in_gaps(dev):  # noqa: F811
+    """h_last between the steps of an f of many rows is taken, one element further into it refused; a step's h may be its own f or x and not its own o"""
+    from apex_amd import _lib, engine
+    lib = _lib.load()
+    B, gap = 2500, 2600
+    mem = torch.randn(2 * (2 * B + gap))
+    f = mem.as_strided((2, B, 1), (2 * B + gap, 2, 1))
+    x, y = torch.randn(2, B, 1), torch.zeros(2, B, 1)
+    want, state = engine.gated_scan(f.clone(), x)
+    for at, ok in ((2 * B, True), (2 * B + gap - B, True), (2 * B - 2, False), (2 * B + gap - B + 1, False), (2 * B - 1, True)):      # (the last row's element is followed by one of the gap)
+        a = _lib.GatedScanArgs(type=0, H=1, T=2, B=B, f=f.data_ptr(), f_t=2 * B + gap, f_b=2, x=x.data_ptr(), x_t=B, x_b=1, y=y.data_ptr(), y_t=B, y_b=1, h_last=mem.data_ptr() + 4 * at)
+        rc = lib.apx_gated_scan_forward(C.byref(a), None)
+        assert rc == (0 if ok else -1), (at, lib.apx_last_error())
+        if ok:
+            assert torch.equal(y, want) and torch.equal(mem[at:at + B], state.view(-1))
+    f, x, h = torch.randn(3, 8), torch.randn(3, 8), torch.randn(3, 8)
+    for first in (True, False):
+        a, b = h.clone(), h.clone()
+        got = engine.gated_scan_step(a if first else f, x if first else a, a, o=x)
+        ref = engine.gated_scan_step(b.clone() if first else f, x if first else b.clone(), b, o=x)
+        assert torch.equal(got, ref) and torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="overlap"):
+        engine.gated_scan_step(f, x, h, o=h)
