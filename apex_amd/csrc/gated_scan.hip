@@ -131,9 +131,9 @@ template <int VEC> struct Channels {
 // Where an operand's rows lie: an access is a wave's address of the first of its steps (scalar registers) and 32 bits of a lane's own, one addition further with every step.  (64-bit
 // addresses in vector registers took 32 of them and two instructions an access, and one in scalar registers for each access more of those than there are.)
 struct Operand {
-    char* base; int64_t step; unsigned lane;
+    char* base; int64_t step; unsigned lane;      // (base as a number: an operand that is not there has none, and is not read)
     template <int VEC> __device__ __forceinline__ Operand(const void* p, const Strides& st, const Channels<VEC>& ch, unsigned bytes)
-        : base((char*)p + ch.b0 * st.b), step(st.t), lane(ch.db * (unsigned)st.b + ch.j * bytes) {}
+        : base((char*)((uintptr_t)p + (uintptr_t)(ch.b0 * st.b))), step(st.t), lane(ch.db * (unsigned)st.b + ch.j * bytes) {}
     __device__ __forceinline__ APX_GLOBAL char* at(int64_t t) const { return wave_address(base + t * step); }
     __device__ __forceinline__ unsigned offset(int i) const { return lane_offset(lane + (unsigned)i * (unsigned)step); }
 };
